@@ -354,6 +354,30 @@ int moe_gather_reduce_rows_peers(const void* const* src_peers, int n_peers, int6
 int moe_scatter_rows(const void* src, int64_t ld_src, const int32_t* row_indx, int64_t n_rows_in, int64_t row_bytes,
                      void* dst, int64_t ld_dst, void* stream);
 
+/* ---- a whole layer for a few tokens --------------------------------------------------------------
+ * y_t = sum over the k largest logits e of (x_t Wg + bg) of softmax weight x (SwiGLU(x_t W1_e + b1_e) W2_e + b2_e) for up to 16 tokens, from x
+ * to y in two kernels; logits, sums and the activation's outputs in fp32, y rounded once.  Equal logits go to the lower expert.  x, y: bf16 or
+ * fp16, rows of d; wg_t: Wg transposed, bf16 [E, d]; b1, b2, bg may be NULL.  W1 [E, d, 2 ff] (gate / linear columns interleaved) and W2
+ * [E, ff, d] in the layout of moe_weight_layout_to_b200.  At most 256 experts, k <= 16, d and ff multiples of 32 up to 8192 (4096 with more
+ * than 8 tokens).  workspace: 256-byte aligned, moe_layer_tokens_workspace_bytes(args) bytes of any contents; calls that may overlap need one
+ * each.  The second kernel is launched cooperatively and takes every SM; its waits are bounded (status codes 1001-1003). */
+typedef struct {
+  const void* x; int x_dtype; int64_t ld_x;
+  int T, d, ff, E, k;
+  const void* wg_t; int64_t ld_wg;
+  const void* bg; int bg_dtype;
+  const void* w1; const void* w1_scale;
+  const void* b1; int b1_dtype; int64_t ld_b1;
+  const void* w2; const void* w2_scale;
+  const void* b2; int b2_dtype; int64_t ld_b2;
+  float act_alpha, act_limit; int act_has_limit;
+  void* y; int y_dtype; int64_t ld_y;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;
+} MoeTokensArgs;
+size_t moe_layer_tokens_workspace_bytes(const MoeTokensArgs* args);
+int moe_layer_tokens(const MoeTokensArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

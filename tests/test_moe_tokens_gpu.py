@@ -1,0 +1,137 @@
+"""`moe_layer_tokens`: a whole MoE layer for a few tokens, against the formula in 64 bits.
+
+The bound of an element is made from the sizes that enter it.  A sum of n fp32 products in any of the kernels' orders is off by at most
+(n / 32 + 64) 2^-23 times the sum of the products' magnitudes (a 32-k group is one exact-product sum of the tensor core, the groups follow one
+another); what is between the sums is carried along by its derivatives; a hidden value as fp16 operand is off by 2^-12 of itself and 2^-25 of
+its row's largest (elements that become subnormal); the result by half a step of its type."""
+import pytest
+import torch
+
+import triton_b200 as tb
+from triton_b200.moe import MoeLayerWeights
+from triton_b200.tensor_details.layout import make_default_matmul_mxfp4_w_layout, make_default_matmul_mxfp4_w_scale_layout
+
+gpu = pytest.mark.gpu
+E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+def make_layer(E, d, ff, seed, device="cuda", alpha=1.702, limit=7.0, bias_dtype=torch.bfloat16):
+    """Random codes and scale bytes straight from a generator -> (MoeLayerWeights, fp64 W1 [E, d, 2 ff], fp64 W2 [E, ff, d])"""
+    g = torch.Generator(device=device).manual_seed(seed)
+
+    def weights(K, N):
+        q = torch.randint(0, 256, (E, N, K // 2), device=device, generator=g, dtype=torch.uint8)
+        s = torch.randint(118, 124, (E, N, K // 32), device=device, generator=g, dtype=torch.uint8)
+        table = torch.tensor(E2M1 + [-v for v in E2M1], dtype=torch.float64, device=device)
+        codes = torch.stack((q & 15, q >> 4), -1).flatten(-2).long()
+        w = table[codes] * torch.exp2(s.double() - 127).repeat_interleave(32, -1)
+        tq = tb.convert_layout(tb.wrap_torch_tensor(q.transpose(1, 2), dtype=tb.FP4), make_default_matmul_mxfp4_w_layout(mx_axis=-2))
+        ts = tb.convert_layout(tb.wrap_torch_tensor(s.transpose(1, 2)), make_default_matmul_mxfp4_w_scale_layout(mx_axis=-2))
+        return tq, ts, w.transpose(1, 2)
+
+    w1, s1, full1 = weights(d, 2 * ff)
+    w2, s2, full2 = weights(ff, d)
+    b1 = (torch.randn(E, 2 * ff, device=device, generator=g) * 0.1).to(bias_dtype)
+    b2 = (torch.randn(E, d, device=device, generator=g) * 0.1).to(bias_dtype)
+    return MoeLayerWeights(w1, s1, b1, w2, s2, b2, alpha, limit), full1, full2
+
+
+def router(d, E, seed, device="cuda", bias=True):
+    g = torch.Generator(device=device).manual_seed(seed + 1000)
+    wg = tb.prepare_router_weight((torch.randn(d, E, device=device, generator=g) / d ** 0.5).bfloat16())
+    return wg, torch.randn(E, device=device, generator=g) if bias else None
+
+
+def reference(x, wg, bg, lw, full1, full2, k):
+    """-> (y, bound) in 64 bits; asserts that the selection is not a matter of rounding"""
+    X, WG = x.double(), wg.double()
+    T, d = X.shape
+    ff = full2.shape[1]
+    lim, al = lw.limit, lw.alpha
+
+    def rounding(n):
+        return (n / 32 + 64) * 2.0 ** -23
+
+    # a logit: a thread's 8 ceil(d / 2048) products one after the other, then 5 steps of a warp, 8 warps and the bias, half a step each
+    router_terms = 8 * -(-d // 2048) + 14
+    b = torch.zeros(wg.shape[1], dtype=torch.float64, device=x.device) if bg is None else bg.double()
+    logits, e_logit = X @ WG + b, router_terms * 2.0 ** -24 * (X.abs() @ WG.abs() + b.abs())
+    vals, indx = torch.sort(logits, dim=1, descending=True, stable=True)
+    if k < logits.shape[1]:
+        gap, err = vals[:, k - 1] - vals[:, k], e_logit.amax(1)
+        assert bool(((gap > 2 * err) | (gap == 0)).all())
+    gates = torch.softmax(vals[:, :k], 1)
+    y, bound = torch.zeros(T, d, dtype=torch.float64, device=x.device), torch.zeros(T, d, dtype=torch.float64, device=x.device)
+    for t in range(T):
+        for j in range(k):
+            e, g = int(indx[t, j]), gates[t, j]
+            pre = X[t] @ full1[e] + lw.b1[e].double()
+            e_pre = rounding(d) * (X[t].abs() @ full1[e].abs() + lw.b1[e].double().abs())
+            gate, lin = pre[0::2], pre[1::2]
+            if lim is not None:
+                gate, lin = gate.clamp(max=lim), lin.clamp(-lim, lim)
+            s = gate * torch.sigmoid(al * gate)
+            h = s * (lin + 1)
+            # |d s / d gate| <= 1.1; the exponential and the division are good to 2^-20 of s
+            e_h = (lin + 1).abs() * (1.1 * e_pre[0::2] + 2.0 ** -20 * s.abs()) + (s.abs() + 1.1 * e_pre[0::2]) * e_pre[1::2]
+            e_h = e_h + 2.0 ** -12 * h.abs() + 2.0 ** -25 * h.abs().max()
+            o = h @ full2[e] + lw.b2[e].double()
+            e_o = e_h @ full2[e].abs() + rounding(ff) * (h.abs() @ full2[e].abs() + lw.b2[e].double().abs())
+            e_gate = 4 * e_logit[t].max() + 2.0 ** -20
+            y[t] += g * o
+            bound[t] += g * (e_o + e_gate * o.abs())
+    return y, bound + (y.abs() + bound) * torch.finfo(x.dtype).eps / 2 + torch.finfo(x.dtype).tiny
+
+
+def check(y, ref, bound):
+    assert torch.isfinite(y).all()
+    off = (y.double() - ref).abs()
+    worst = (off / bound).max().item()
+    assert worst <= 1.0, f"{worst} of the bound"
+
+
+def run_case(T, E, k, d, ff, dtype=torch.bfloat16, seed=0, bias=True, **layer):
+    lw, full1, full2 = make_layer(E, d, ff, seed, **layer)
+    wg, bg = router(d, E, seed, bias=bias)
+    x = torch.randn(T, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed + 7)).to(dtype)
+    y = tb.moe_layer_tokens(x, wg, bg, lw, k)
+    tb.matmul_check_status()
+    assert y.shape == x.shape and y.dtype == dtype
+    ref, bound = reference(x, wg, bg, lw, full1, full2, k)
+    check(y, ref, bound)
+    return x, wg, bg, lw, y
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 13, 16])
+def test_token_counts(T, dtype):
+    run_case(T, 16, 4, 256, 192, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("T,E,k,d,ff", [
+    (1, 1, 1, 32, 32),              # one unit, one stage, one expert
+    (16, 1, 1, 32, 64),             # every token at one expert
+    (1, 2, 2, 512, 1024),           # fewer stages than SMs
+    (3, 5, 3, 736, 1440),           # extents that end inside tiles
+    (7, 8, 8, 96, 160),             # every expert of every token
+    (16, 16, 16, 64, 96),
+    (2, 256, 16, 64, 32),
+    (16, 255, 7, 128, 96),
+    (4, 8, 2, 2880, 2880),
+    (16, 12, 4, 1024, 544),
+    (8, 2, 2, 8192, 32),            # the widest
+    (8, 2, 1, 32, 8192),
+    (16, 3, 2, 4096, 64),
+    (9, 3, 2, 64, 4096),
+])
+def test_shapes(T, E, k, d, ff):
+    run_case(T, E, k, d, ff, seed=3)
+
+
+@gpu
+def test_without_router_bias_and_with_other_activation():
+    run_case(3, 8, 2, 256, 256, bias=False)
+    run_case(3, 8, 2, 256, 256, limit=None, alpha=1.0, seed=5)
+    run_case(3, 8, 2, 256, 256, bias_dtype=torch.float32, limit=0.5, seed=6)

@@ -4,6 +4,7 @@
 // binding loaded (its handle is passed in), and every entry point keeps its checks and messages.
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include "../../include/moe_b200.h"
@@ -19,7 +20,7 @@ struct Lib {
   X(moe_last_error) X(moe_route) X(moe_route_positions) X(moe_route_workspace) X(moe_grouped_gemm) X(moe_gemm_mx_workspace_bytes) \
   X(moe_reduce) X(moe_downcast_mxfp4) X(moe_upcast_mxfp4) X(moe_bitmatrix_metadata) X(moe_bitmatrix_metadata_workspace) \
   X(moe_router_topk) X(moe_copy2) X(moe_step_graph_create) X(moe_step_graph_launch) X(moe_step_graph_destroy) \
-  X(moe_gemm_kernel_name) X(moe_grouped_gemm_chain)
+  X(moe_gemm_kernel_name) X(moe_grouped_gemm_chain) X(moe_layer_tokens) X(moe_layer_tokens_workspace_bytes)
 #define X(name) decltype(&::name) name = nullptr;
   MOE_HOST_FUNCTIONS(X)
 #undef X
@@ -332,6 +333,48 @@ Tensor layer(const Tensor& x, const Tensor& logits, int64_t k, const py::tuple& 
   return z;
 }
 
+// ---- a whole layer for a few tokens --------------------------------------------------------------------------------
+void same_device(const Tensor& x, const Tensor& t, const char* what) {
+  if (t.device() != x.device()) raise(PyExc_ValueError, std::string(what) + " is on " + t.device().str() + ", x on " + x.device().str());
+}
+// a matrix whose rows the kernels load 16 bytes at a time: as it is, or copied
+Tensor aligned_rows(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  return t.stride(1) == 1 && (t.size(0) < 2 || t.stride(0) % per == 0) && (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// w1, w2: (values, scales, bias) in the default tiles; the work runs on x's device, on its current stream
+Tensor moe_tokens(const Tensor& x_, const Tensor& wg, const OptTensor& bg, int64_t k, const py::tuple& w1, const py::tuple& w2, int64_t ff, double alpha,
+                  std::optional<double> limit, const Tensor& status) {
+  need_cuda(x_);
+  const c10::cuda::CUDAGuard guard(x_.device());
+  const Tensor x = aligned_rows(x_);
+  MoeTokensArgs g{};
+  g.x = x.data_ptr(); g.x_dtype = g.y_dtype = dtype_code(x); g.ld_x = x.size(0) > 1 ? x.stride(0) : x.size(1);
+  g.T = (int)x.size(0); g.d = (int)x.size(1); g.ff = (int)ff; g.E = (int)wg.size(1); g.k = (int)k;
+  same_device(x, wg, "wg");
+  g.wg_t = wg.data_ptr(); g.ld_wg = wg.size(1) > 1 ? wg.stride(1) : wg.size(0);
+  if (bg) { same_device(x, *bg, "bg"); g.bg = bg->data_ptr(); g.bg_dtype = dtype_code(*bg); }
+  const Tensor v1 = w1[0].cast<Tensor>(), s1 = w1[1].cast<Tensor>(), b1 = w1[2].cast<Tensor>();
+  const Tensor v2 = w2[0].cast<Tensor>(), s2 = w2[1].cast<Tensor>(), b2 = w2[2].cast<Tensor>();
+  for (const Tensor* t : {&v1, &s1, &b1, &v2, &s2, &b2}) same_device(x, *t, "a weight");
+  same_device(x, status, "the status word");
+  g.w1 = v1.data_ptr(); g.w1_scale = s1.data_ptr(); g.b1 = b1.data_ptr(); g.b1_dtype = dtype_code(b1); g.ld_b1 = b1.stride(0);
+  g.w2 = v2.data_ptr(); g.w2_scale = s2.data_ptr(); g.b2 = b2.data_ptr(); g.b2_dtype = dtype_code(b2); g.ld_b2 = b2.stride(0);
+  g.act_alpha = (float)alpha;
+  if (limit) { g.act_limit = (float)*limit; g.act_has_limit = 1; }
+  Tensor y = empty({g.T, g.d}, x.scalar_type(), x);
+  if (g.T == 0) return y;
+  g.y = y.data_ptr(); g.ld_y = g.d;
+  g.workspace_bytes = lib.moe_layer_tokens_workspace_bytes(&g);
+  if (g.workspace_bytes == 0) check(3, "moe_layer_tokens");       // sizes it does not take: its message
+  const Tensor ws = empty({(int64_t)g.workspace_bytes}, at::kByte, x);
+  g.workspace = ws.data_ptr();
+  g.status = status.data_ptr<int32_t>();
+  check(lib.moe_layer_tokens(&g, stream()), "moe_layer_tokens");
+  return y;
+}
+
 // ---- quantiser, combine --------------------------------------------------------------------------------------------
 // [batch, outer, quant] element strides of `t` with its last axis quantised; false when the leading axes do not merge into two
 bool collapse3(const Tensor& t, int64_t (&e)[2], int64_t (&s)[2]) {
@@ -497,6 +540,7 @@ PYBIND11_MODULE(_host, m) {
   m.def("gemm_kernel", &gemm_kernel, py::arg("kind"), py::arg("E"), py::arg("K"), py::arg("N"), py::arg("M"), py::arg("x_dtype"),
         py::arg("y_dtype"), py::arg("tuning"), py::arg("rows_per_expert") = 0, py::arg("swiglu") = false);
   m.def("layer", &layer);
+  m.def("moe_tokens", &moe_tokens);
   m.def("downcast", &downcast);
   m.def("upcast", &upcast);
   m.def("reduce", &reduce);

@@ -127,6 +127,8 @@ _STATUS_TEXT = {
     801: "router kernel: the producer waited for a free stage", 802: "router kernel: the MMA thread waited for a stage",
     803: "router kernel: the MMA warp waited for a free accumulator", 804: "router kernel: the selection waited for the accumulator",
     901: "expert-parallel peer barrier: a rank did not arrive within the limit; the step after it read stale peer buffers",
+    1001: "layer of a few tokens: the weight producer waited for a free stage", 1002: "layer of a few tokens: a warp waited for weights",
+    1003: "layer of a few tokens: fc2 waited for fc1's rows",
 }
 
 
@@ -137,7 +139,7 @@ def status_message(code: int) -> str:
 
 def matmul_check_status(device=None):
     """Synchronise and raise if a bounded wait expired since the last check: a pipeline wait inside a tensor-core
-    kernel (codes 1xx-8xx) or an expert-parallel peer barrier (901).  Expert-parallel callers should poll this once
+    kernel (codes 1xx-8xx and 10xx) or an expert-parallel peer barrier (901).  Expert-parallel callers should poll this once
     per step or batch: after a barrier time-out the step carries on with stale peer buffers and its result is wrong."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     w = _status_word(dev)
