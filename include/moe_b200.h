@@ -360,7 +360,7 @@ int moe_scatter_rows(const void* src, int64_t ld_src, const int32_t* row_indx, i
  * fp16, rows of d; wg_t: Wg transposed, bf16 [E, d]; b1, b2, bg may be NULL.  W1 [E, d, 2 ff] (gate / linear columns interleaved) and W2
  * [E, ff, d] in the layout of moe_weight_layout_to_b200.  At most 256 experts, k <= 16, d and ff multiples of 32 up to 8192 (4096 with more
  * than 8 tokens).  workspace: 256-byte aligned, moe_layer_tokens_workspace_bytes(args) bytes of any contents; calls that may overlap need one
- * each.  The second kernel is launched cooperatively and takes every SM; its waits are bounded (status codes 1001-1003). */
+ * each.  The second kernel is launched cooperatively and takes every SM; its waits are bounded (status codes 1001-1006). */
 typedef struct {
   const void* x; int x_dtype; int64_t ld_x;
   int T, d, ff, E, k;

@@ -2,8 +2,8 @@
 
 The bound of an element is made from the sizes that enter it.  A sum of n fp32 products in any of the kernels' orders is off by at most
 (n / 32 + 64) 2^-23 times the sum of the products' magnitudes (a 32-k group is one exact-product sum of the tensor core, the groups follow one
-another); what is between the sums is carried along by its derivatives; a hidden value as fp16 operand is off by 2^-12 of itself and 2^-25 of
-its row's largest (elements that become subnormal); the result by half a step of its type."""
+another); what is between the sums is carried along by its derivatives; a hidden value as fp16 operand is off by 2^-12 of itself and 2^-24 of
+its row's largest (elements that become subnormal), a token by the latter; the result by half a step of its type."""
 import pytest
 import torch
 
@@ -67,6 +67,7 @@ def reference(x, wg, bg, lw, full1, full2, k):
             e, g = int(indx[t, j]), gates[t, j]
             pre = X[t] @ full1[e] + lw.b1[e].double()
             e_pre = rounding(d) * (X[t].abs() @ full1[e].abs() + lw.b1[e].double().abs())
+            e_pre = e_pre + 2.0 ** -24 * X[t].abs().max() * full1[e].abs().sum(0)
             gate, lin = pre[0::2], pre[1::2]
             if lim is not None:
                 gate, lin = gate.clamp(max=lim), lin.clamp(-lim, lim)
@@ -74,7 +75,7 @@ def reference(x, wg, bg, lw, full1, full2, k):
             h = s * (lin + 1)
             # |d s / d gate| <= 1.1; the exponential and the division are good to 2^-20 of s
             e_h = (lin + 1).abs() * (1.1 * e_pre[0::2] + 2.0 ** -20 * s.abs()) + (s.abs() + 1.1 * e_pre[0::2]) * e_pre[1::2]
-            e_h = e_h + 2.0 ** -12 * h.abs() + 2.0 ** -25 * h.abs().max()
+            e_h = e_h + 2.0 ** -12 * h.abs() + 2.0 ** -24 * h.abs().max()
             o = h @ full2[e] + lw.b2[e].double()
             e_o = e_h @ full2[e].abs() + rounding(ff) * (h.abs() @ full2[e].abs() + lw.b2[e].double().abs())
             e_gate = 4 * e_logit[t].max() + 2.0 ** -20

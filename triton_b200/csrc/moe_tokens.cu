@@ -6,21 +6,22 @@
 // steps that depend on one another.  Hence two kernels, and few waits in the second:
 //  1. moe_tokens_router_kernel, a CTA per expert: its logit of every token, on CUDA cores (an expert's row of Wg is 6 KB: nothing to tile).
 //  2. moe_tokens_kernel, one CTA per SM, launched cooperatively.  Every CTA selects the k best of every token for itself (a warp per token), so that the
-//     list of active experts needs no exchange.  Weights are cut into units of 32 rows over all of k; a unit is streamed in stages of 512 k (one
+//     list of active experts needs no exchange.  Weights are cut into units of 32 rows over all of k; a unit is streamed in stages of 1024 k (one
 //     TMA box of values, one of scales) by one thread through a ring that takes what shared memory is left.  fc1's units are dealt out evenly, and fc2's
 //     stages, whose sums may be cut anywhere.  fc2 reads all of fc1's outputs of an expert: a counter per expert in global memory says when they are
 //     there, and the ring goes on filling with fc2's weights meanwhile (one token of four experts: all of them).
-//     fc2's partial sums go to the workspace; a counter per 32 output columns tells the CTA whose contribution completes them, which adds them up in
-//     a fixed order (slots, then parts along k): the result does not depend on who comes last.
+//     fc2's partial sums go to the workspace; a counter per 32 output columns says when they are complete, and a warp of whichever CTA adds up 32
+//     outputs of a token in a fixed order (slots, then parts along k): the result does not depend on who comes last.
 //
-// Arithmetic: a code converts to fp16 exactly (two codes an instruction), tokens are fp16 scaled by a power of two per row that puts the largest
-// finite element in [2^11, 2^12): elements down to 2^-25 of it keep all of bf16's bits.  mma.sync m16n8k16 sums one scale group of 32 k in fp32, which
+// Arithmetic: a code becomes fp16 exactly, tokens are fp16 scaled by their row's largest finite element, which is put in [2^13, 2^14):
+// elements down to 2^-30 of it keep all of bf16's bits.  mma.sync m16n8k16 sums one scale group of 32 k in fp32, which
 // is multiplied by the group's scale and added up in fp32.  The legacy tensor path is far more than 16 tokens need, and its fragments come straight
 // from the packed words.  SwiGLU outputs stay fp32 in the workspace; as operand they are fp16 of the row's scale, 2^-12 of a value off, in two terms
 // (2^-23) where the expert has at most half as many tokens as there are columns.
 #include "gemm_tc_common.cuh"
 #include "topk_select.cuh"
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace {
 
@@ -29,18 +30,21 @@ constexpr int MT_MAX_K = 16;              // picks per token
 constexpr int MT_MAX_EXPERTS = 256;
 constexpr int MT_WARPS = 16;              // consumer warps: 8 shares of k times 2 slabs of 16 weight rows
 constexpr int MT_CONSUMERS = MT_WARPS * 32;
-constexpr int MT_THREADS = MT_CONSUMERS + 32;
+constexpr int MT_EPILOGUE = 96;           // threads that take the sums on while the consumers are at the next unit
+constexpr int MT_THREADS = MT_CONSUMERS + MT_EPILOGUE + 32;
 constexpr int MT_UNIT = 32;               // weight rows of a unit
-constexpr int MT_STAGE_KT = 4;            // 128-k tiles of a stage
+constexpr int MT_STAGE_KT = 8;            // 128-k tiles of a stage, one per share of k
 constexpr int MT_STAGE_VALUES = MT_STAGE_KT * 4 * MT_UNIT * 16;
 constexpr int MT_STAGE_BYTES = MT_STAGE_VALUES + MT_STAGE_KT * MT_UNIT * 4;
-constexpr int MT_MAX_STAGES = 24;
+constexpr int MT_RED_LD = 36;             // pitch of a column of sums: the quads of an accumulator fragment go to distinct banks
+constexpr int MT_MAX_STAGES = 12;
 constexpr int MT_COUNTERS = 256;          // words of each of the three counter arrays
 constexpr int MT_ROUTER_THREADS = 256;
 
 struct TokensParams {
   const void* x; int x_dtype; int64_t ld_x;
   int T, d, ff, E, k;
+  const uint8_t* s1; const uint8_t* s2;
   const void* b1; int b1_dtype; int64_t ld_b1;
   const void* b2; int b2_dtype; int64_t ld_b2;
   float alpha, limit; int has_limit;
@@ -127,20 +131,42 @@ moe_tokens_router_kernel(const TX* x, int64_t ld_x, int T, int d, const __nv_bfl
 }
 
 // ---- layer -----------------------------------------------------------------------------------------------------
-// e2m1 codes of a word -> fp16 pairs: byte b holds k = (0, 2), (4, 6), (1, 3), (5, 7) of its eight
+// The eight e2m1 codes of a word (nibbles k0, k2, k4, k6 | k1, k3, k5, k7, lowest first) -> fp16 pairs (0, 2), (4, 6), (1, 3), (5, 7), exactly.  A stage
+// took 524 cycles of an SM this way (its bytes take some 750 from HBM), 760 with half of the pairs made by shifts and masks and 967 with all.
 __device__ __forceinline__ void e2m1_word(uint32_t w, uint32_t (&h)[4]) {
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\tcvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// e8m0 byte -> 2^(byte - 127): byte 0 is 0.0 and byte 255 is NaN, as the dequantiser has them
-__device__ __forceinline__ float e8m0_f32(uint32_t b) { return __uint_as_float((b << 23) | ((b + 1u) >> 8)); }
-// power of two that puts the largest finite element of a row in [2^11, 2^12)
-__device__ __forceinline__ int row_exponent(float mx) { return max(-126, min(116, (int)(__float_as_uint(mx) >> 23) - 127 - 11)); }
+// four e8m0 bytes -> 2^(byte - 127): byte 0 is 0.0 as the dequantiser has it; byte 255, there NaN, gives infinity, which settle() takes up
+__device__ __forceinline__ void e8m0_word(uint32_t w, float (&f)[4]) {
+  f[0] = __uint_as_float((w << 23) & 0x7F800000u);
+  f[1] = __uint_as_float((w << 15) & 0x7F800000u);
+  f[2] = __uint_as_float((w << 7) & 0x7F800000u);
+  f[3] = __uint_as_float((w >> 1) & 0x7F800000u);
+}
+// A sum over weight row `row` of expert e: a scale byte of 255 anywhere in the row makes it NaN.  Such a sum has become infinite (or NaN: a group of zeros),
+// so only those look at the scales again.
+__device__ __forceinline__ float settle(float v, const uint8_t* scales, int e, int NT, int KT, int row) {
+  if (fabsf(v) == __int_as_float(0x7F800000)) {
+    const uint8_t* at = scales + ((int64_t)(e * NT + (row >> 7)) * KT) * 512 + (row & 127) * 4;
+    for (int kt = 0; kt < KT; ++kt) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(at + (int64_t)kt * 512);
+      if (((w & 0x7F7F7F7Fu) + 0x01010101u) & w & 0x80808080u) return __int_as_float(0x7FC00000);
+    }
+  }
+  return v;
+}
+// Exponent of the largest finite element of a row.  Its values as operands are scaled by 2^(13 - exponent): the largest in [2^13, 2^14).
+__device__ __forceinline__ int row_exponent(float mx) { return max(-112, min(126, (int)(__float_as_uint(mx) >> 23) - 127)); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -165,23 +191,52 @@ __device__ __forceinline__ int ld_acquire(const int32_t* p) {
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
-static_assert(MT_CONSUMERS == 512, "consumer_bar");
+// until the counter has got to `full`; bounded like mbar_wait
+__device__ __forceinline__ bool wait_count(const int32_t* counter, int full, const Ctl& ctl, int code) {
+  if (ld_acquire(counter) >= full) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 0;; ++i) {
+    if (ld_acquire(counter) >= full) return true;
+    if ((i & 7u) == 7u && *ctl.abort_flag) return false;
+    if ((i & 255u) == 255u && clock64() - t0 > WAIT_LIMIT_CYCLES) {
+      *ctl.abort_flag = 1;
+      if (ctl.status) atomicExch(ctl.status, code);
+      return false;
+    }
+  }
+}
+// mbar_wait for the loops of few instructions: what is hardly ever run is a call, and time is counted in tries (each of which may take a while)
+__device__ __noinline__ bool mbar_expired(uint32_t tries, const Ctl ctl, int code) {
+  if (*ctl.abort_flag) return true;
+  if (tries < (1u << 24)) return false;
+  *ctl.abort_flag = 1;
+  if (ctl.status) atomicExch(ctl.status, code);
+  return true;
+}
+__device__ __forceinline__ void mbar_wait_short(uint32_t bar, uint32_t parity, const Ctl& ctl, int code) {
+  uint32_t tries = 0;
+  while (!mbar_try(bar, parity))
+    if ((++tries & 1023u) == 0 && mbar_expired(tries, ctl, code)) break;
+}
+// named barriers: 1 consumers, 2 epilogue
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+constexpr int MT_BOTH = MT_CONSUMERS + MT_EPILOGUE;
 
 struct TokensShared {                   // beside ring, staged tokens and partial sums
   uint64_t full[MT_MAX_STAGES], empty[MT_MAX_STAGES];
+  uint64_t sums[2], taken[2];           // a buffer of sums is complete, has been read
   int abort;
   int n_active;
   int counts[8];
   int act[MT_MAX_EXPERTS];              // active experts in ascending order
   uint16_t rank[MT_MAX_EXPERTS];        // place of an expert in that list
   uint16_t tokens[MT_MAX_EXPERTS];      // its tokens, a bit each
-  alignas(16) uint8_t slot[MT_MAX_EXPERTS][MT_MAX_TOKENS];     // which pick of the token it is
+  alignas(16) uint8_t slot[MT_MAX_EXPERTS][MT_MAX_TOKENS];     // which pick of the token it is, 255: none
+  uint8_t who[MT_MAX_EXPERTS][MT_MAX_TOKENS];      // its tokens one behind the other
   uint8_t sel[MT_MAX_TOKENS][MT_MAX_K];
   float gate[MT_MAX_TOKENS][MT_MAX_K];
-  float undo[MT_MAX_TOKENS];            // 2^exponent of the staged rows
-  int n_done;
-  int done[MT_COUNTERS];
+  float undo1[MT_MAX_TOKENS];           // what the sums over staged rows are short of: of fc1's tokens, of fc2's last four experts
+  float undo2[4][MT_MAX_TOKENS];
 };
 
 // A warp selects the k largest logits of token t, ties to the lower expert, and their softmax
@@ -214,16 +269,95 @@ __device__ __forceinline__ void select_token(const TokensParams& p, TokensShared
   if (lane < p.k) s.gate[t][lane] = __fdiv_rn(mine, sum);
 }
 
+// staged token column col, eight k from 8 * k8 on
+__device__ __forceinline__ uint32_t tok_at(uint32_t toks, int nblk, int col, int k8) {
+  return toks + (uint32_t)((((k8 >> 2) * nblk + (col >> 3)) * 8 + (col & 7)) * 64 + (k8 & 3) * 16);
+}
+// token t as a column of fc1, by a warp: chunks of 256 k, six of them on their way at a time
+__device__ __forceinline__ void stage_x(const TokensParams& p, TokensShared& s, int nblk, uint32_t toks, int t) {
+  const int lane = threadIdx.x & 31, end = ((p.d + 127) >> 7) * 16;
+  const int ex = row_exponent(__ldcg(p.xmax + t));
+  const float scale = pow2(13 - ex);
+  for (int k0 = lane; k0 < end; k0 += 6 * 32) {
+    uint4 raw[6];
+#pragma unroll
+    for (int u = 0; u < 6; ++u) {
+      const int k8 = k0 + u * 32;
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (k8 * 8 < p.d) raw[u] = *reinterpret_cast<const uint4*>((const uint16_t*)p.x + t * p.ld_x + k8 * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < 6; ++u) {
+      const int k8 = k0 + u * 32;
+      if (k8 >= end) break;
+      const uint16_t* e = reinterpret_cast<const uint16_t*>(&raw[u]);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = (p.x_dtype == MOE_F16 ? __half2float(__ushort_as_half(e[j])) : __uint_as_float((uint32_t)e[j] << 16)) * scale;
+      sts128(tok_at(toks, nblk, t, k8), pack8(v));
+    }
+  }
+  if (lane == 0) s.undo1[t] = pow2(ex - 13);
+}
+// whether an expert's rows are staged in two terms
+__device__ __forceinline__ bool two_terms(int n, int nblk) { return 2 * n <= 8 * nblk; }
+
+// An expert's hidden rows as the columns of fc2 (n of them), behind one another, their second terms behind the first: a warp takes 256 k of a row,
+// two at a time
+__device__ __forceinline__ void stage_h(const TokensParams& p, TokensShared& s, int nblk, uint32_t toks, int e, int n, int KT2, int place, int warp) {
+  const int lane = threadIdx.x & 31;
+  const bool two = two_terms(n, nblk);
+  const int chunks = (KT2 + 1) >> 1, total = n * chunks;
+  for (int i0 = warp; i0 < total; i0 += 2 * MT_WARPS) {   // 256 k of a row by a warp, two at a time
+    float4 raw[2][2];
+    float mx[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int i = i0 + x * MT_WARPS, r = i / chunks, k8 = (i - r * chunks) * 32 + lane;
+      raw[x][0] = raw[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      mx[x] = 0.0f;
+      if (i < total) {
+        const int t = s.who[e][r], entry = t * p.k + s.slot[e][t];
+        mx[x] = __uint_as_float(__ldcg(p.hmax + entry));
+        if (k8 * 8 < p.ff) {
+          const float4* src = reinterpret_cast<const float4*>(p.h + (int64_t)entry * p.ff + k8 * 8);
+          raw[x][0] = __ldcg(src);
+          raw[x][1] = __ldcg(src + 1);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int i = i0 + x * MT_WARPS, r = i / chunks, k8 = (i - r * chunks) * 32 + lane;
+      if (i >= total || k8 >= KT2 * 16) continue;
+      const int ex = row_exponent(mx[x]);
+      float v[8] = {raw[x][0].x, raw[x][0].y, raw[x][0].z, raw[x][0].w, raw[x][1].x, raw[x][1].y, raw[x][1].z, raw[x][1].w}, w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] *= pow2(13 - ex);
+        const float left = v[j] - __half2float(__float2half_rn(v[j]));     // (infinities and NaN are the first term's)
+        w[j] = isfinite(left) ? left : 0.0f;
+      }
+      sts128(tok_at(toks, nblk, r, k8), pack8(v));
+      if (two) sts128(tok_at(toks, nblk, n + r, k8), pack8(w));
+      if (k8 == 0) s.undo2[place][r] = pow2(ex - 13);
+    }
+  }
+}
+
 template <int NBLK>                     // blocks of eight token columns
 __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensParams p, const __grid_constant__ TokensMaps maps) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
   __shared__ TokensShared s;
-  __shared__ __align__(16) float s_red[2][8][2 * NBLK * 128];          // [buffer][share of k][slab, block, lane, 4]
+  __shared__ __align__(16) float s_red[2][8][8 * NBLK * MT_RED_LD];    // [buffer][share of k][column][row]
   const uint32_t ring = smem_u32(smem), toks = ring + (uint32_t)(p.stages * MT_STAGE_BYTES);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;     // warp-uniform for the compiler
   auto FULL = [&](int i) { return smem_u32(&s.full[i]); };
   auto EMPTY = [&](int i) { return smem_u32(&s.empty[i]); };
+  auto SUMS = [&](int i) { return smem_u32(&s.sums[i]); };
+  auto TAKEN = [&](int i) { return smem_u32(&s.taken[i]); };
   const Ctl ctl{&s.abort, p.status};
 
   if (threadIdx.x == 0) {
@@ -231,12 +365,16 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
       mbar_init(FULL(i), 1);
       mbar_init(EMPTY(i), MT_WARPS);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(SUMS(i), MT_WARPS);
+      mbar_init(TAKEN(i), MT_EPILOGUE / 32);
+    }
     s.abort = 0;
-    s.n_done = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (threadIdx.x < MT_MAX_EXPERTS) *reinterpret_cast<uint4*>(s.slot[threadIdx.x]) = make_uint4(~0u, ~0u, ~0u, ~0u);
   if (warp < p.T) select_token(p, s, warp, lane);
+  else if (NBLK == 1 && warp >= 8 && warp - 8 < p.T) stage_x(p, s, NBLK, toks, warp - 8);
   __syncthreads();
   if (threadIdx.x < p.T * p.k) {
     const int t = threadIdx.x / p.k, j = threadIdx.x - t * p.k;
@@ -248,7 +386,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     const int e = threadIdx.x;
     if (e < MT_MAX_EXPERTS) {
 #pragma unroll
-      for (int t = 0; t < MT_MAX_TOKENS; ++t) mask |= (s.slot[e][t] != 0xFF ? 1u : 0u) << t;
+      for (int t = 0; t < MT_MAX_TOKENS; ++t)
+        if (s.slot[e][t] != 0xFF) {
+          s.who[e][__popc(mask)] = (uint8_t)t;
+          mask |= 1u << t;
+        }
       s.tokens[e] = (uint16_t)mask;
     }
     const uint32_t live = __ballot_sync(0xFFFFFFFFu, mask != 0);
@@ -265,260 +407,302 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
 
   const int A = s.n_active, G = gridDim.x, c = blockIdx.x;
   const int KT1 = (p.d + 127) >> 7, KT2 = (p.ff + 127) >> 7, KS1 = (KT1 + MT_STAGE_KT - 1) / MT_STAGE_KT, KS2 = (KT2 + MT_STAGE_KT - 1) / MT_STAGE_KT;
-  const int NB1 = 2 * p.ff / MT_UNIT, NB2 = p.d / MT_UNIT;
+  const int NB1 = 2 * p.ff / MT_UNIT, NB2 = p.d / MT_UNIT, NT1 = (2 * p.ff + 127) >> 7, NT2 = (p.d + 127) >> 7;
   const int U1 = A * NB1;
-  const int64_t S2 = (int64_t)A * NB2 * KS2;
-  const int u_begin = (int)((int64_t)U1 * c / G), u_end = (int)((int64_t)U1 * (c + 1) / G);
-  const int64_t s_begin = S2 * c / G, s_end = S2 * (c + 1) / G;
+  const int S2 = A * NB2 * KS2;                              // (times the CTAs it stays below 2^31: 2^19 * 148)
+  const int u_begin = U1 * c / G, u_end = U1 * (c + 1) / G, s_begin = S2 * c / G, s_end = S2 * (c + 1) / G;
+  const int first2 = s_begin / KS2, n1 = u_end - u_begin, n2 = s_end > s_begin ? (s_end - 1) / KS2 - first2 + 1 : 0;      // units here
 
-  if (warp == MT_WARPS) {
+  if (warp == MT_BOTH / 32) {
     // ================================= weights =================================================================
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      auto stage = [&](const CUtensorMap* v, const CUtensorMap* sc, int tiles, int nb, int64_t tile) {
-        const int i = it % p.stages;
-        ok = mbar_wait(EMPTY(i), ((it / p.stages) & 1u) ^ 1u, ctl, 1001);
-        if (!ok) return;
-        const uint32_t dst = ring + (uint32_t)(i * MT_STAGE_BYTES);
-        mbar_expect_tx(FULL(i), (uint32_t)(tiles * MT_UNIT * 68));
-        tma_tile_2d(dst, v, (nb & 3) * 128, (int)(tile * 4), FULL(i));
-        tma_tile_2d(dst + MT_STAGE_VALUES, sc, (nb & 3) * 32, (int)tile, FULL(i));
-        ++it;
-      };
-      const int NT1 = (2 * p.ff + 127) >> 7, NT2 = (p.d + 127) >> 7;
-      const int tail1 = KT1 - (KS1 - 1) * MT_STAGE_KT, tail2 = KT2 - (KS2 - 1) * MT_STAGE_KT;
-      for (int u = u_begin; u < u_end && ok; ++u) {
-        const int a = u / NB1, nb = u - a * NB1;
-        const int64_t tile = ((int64_t)s.act[a] * NT1 + (nb >> 2)) * KT1;
-        for (int js = 0; js < KS1 && ok; ++js) {
-          if (js < KS1 - 1) stage(&maps.v1, &maps.s1, MT_STAGE_KT, nb, tile + js * MT_STAGE_KT);
-          else stage(&maps.v1t, &maps.s1t, tail1, nb, tile + js * MT_STAGE_KT);
+    // the warp goes through the loop as a whole and elects a lane at each instruction: a thread by itself took longer to issue a stage's copies
+    // than they take from HBM
+    int ri = 0;
+    uint32_t rp = 1, it = 0;
+    bool ok = true;
+    auto stage = [&](const CUtensorMap* v, const CUtensorMap* sc, uint32_t bytes, int nb, int tile) {
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(ri), rp, ctl, 1001));
+      if (!ok) return;
+      const uint32_t dst = ring + (uint32_t)(ri * MT_STAGE_BYTES);
+      elect_expect_tx(FULL(ri), bytes);
+      elect_tile_2d(dst, v, (nb & 3) * 128, tile * 4, FULL(ri));
+      elect_tile_2d(dst + MT_STAGE_VALUES, sc, (nb & 3) * 32, tile, FULL(ri));
+      if (++ri == p.stages) { ri = 0; rp ^= 1u; }
+      ++it;
+    };
+    // units [from, from + units) of a product, their stages from js0 in the first to js1 in the last
+    auto product = [&](const CUtensorMap* v, const CUtensorMap* sc, const CUtensorMap* vt, const CUtensorMap* st, int NB, int NT, int KT, int KS, int from,
+                       int units, int js0, int js1) {
+      const uint32_t whole = MT_STAGE_KT * MT_UNIT * 68, tail = (uint32_t)((KT - (KS - 1) * MT_STAGE_KT) * MT_UNIT * 68);
+      int place = from / NB, nb = from - place * NB;
+#pragma unroll 1
+      for (int m = 0; m < units && ok; ++m) {
+        const int tile = (s.act[place] * NT + (nb >> 2)) * KT, end = m + 1 == units ? js1 : KS;
+#pragma unroll 1
+        for (int js = m == 0 ? js0 : 0; js < end && ok; ++js) {
+          if (js < KS - 1) stage(v, sc, whole, nb, tile + js * MT_STAGE_KT);
+          else stage(vt, st, tail, nb, tile + js * MT_STAGE_KT);
+        }
+        if (++nb == NB) { nb = 0; ++place; }
+      }
+    };
+    product(&maps.v1, &maps.s1, &maps.v1t, &maps.s1t, NB1, NT1, KT1, KS1, u_begin, n1, 0, KS1);
+    product(&maps.v2, &maps.s2, &maps.v2t, &maps.s2t, NB2, NT2, KT2, KS2, first2, n2, s_begin - first2 * KS2, s_end - (first2 + n2 - 1) * KS2);
+    if (!ok && lane == 0) {                                   // copies in flight land before the block's shared memory goes
+      const uint32_t lo = it > (uint32_t)p.stages ? it - p.stages : 0;
+      for (uint32_t j = lo; j < it; ++j)
+        for (uint32_t t = 0; t < (1u << 16) && !mbar_test(FULL(j % p.stages), (j / p.stages) & 1u); ++t) __nanosleep(64);
+    }
+    return;
+  }
+
+  if (warp >= MT_WARPS) {
+    // ================================= epilogue ================================================================
+    const int tid = threadIdx.x - MT_CONSUMERS;
+    int a = u_begin / NB1, nb = u_begin - a * NB1;            // of the unit
+    const int i = tid & 15;
+    // the bias of a unit is asked for while the one before is at work: its way from memory is longer than a unit's
+    float bias[2] = {0.0f, 0.0f};
+    auto ask = [&](int a, int nb) {
+      if (p.b1 && a < A) {
+        const int64_t at = s.act[a] * p.ld_b1 + 2 * (nb * 16 + i);
+        bias[0] = load_bias(p.b1, p.b1_dtype, at);
+        bias[1] = load_bias(p.b1, p.b1_dtype, at + 1);
+      }
+    };
+    ask(a, nb);
+    constexpr int STEP = MT_EPILOGUE / 16, ROUNDS = (8 * NBLK + STEP - 1) / STEP;
+    float top[ROUNDS];                                        // largest output of each of the thread's tokens in this expert's units so far
+#pragma unroll
+    for (int q = 0; q < ROUNDS; ++q) top[q] = 0.0f;
+#pragma unroll 1
+    for (int m = 0; m < n1; ++m) {
+      const int e = s.act[a], n = __popc(s.tokens[e]), o = nb * 16 + i, was = nb;
+      const float bg = bias[0], bl = bias[1];
+      if (++nb == NB1) { nb = 0; ++a; }
+      ask(a, nb);
+      mbar_wait_short(SUMS(m & 1), (m >> 1) & 1u, ctl, 1005);
+      // sixteen outputs of a token by half a warp, MT_EPILOGUE / 16 tokens at a time
+      const int r0 = tid >> 4, mine = (n - (tid >> 5 << 1) + STEP - 1) / STEP;       // rounds of this warp
+      if (mine <= 0 && (tid & 31) == 0) mbar_arrive(TAKEN(m & 1));
+#pragma unroll
+      for (int q = 0; q < ROUNDS; ++q) {
+        if (q >= mine) break;
+        const int r = r0 + q * STEP;
+        const bool live = r < n;
+        const int t = s.who[e][live ? r : 0], entry = t * p.k + s.slot[e][t];
+        float g = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(&s_red[m & 1][w][t * MT_RED_LD + 2 * i]);
+          g += v.x;
+          l += v.y;
+        }
+        if (q + 1 == mine) {                                  // the buffer may be filled again
+          __syncwarp();
+          if ((tid & 31) == 0) mbar_arrive(TAKEN(m & 1));
+        }
+        g = fmaf(settle(g, p.s1, e, NT1, KT1, 2 * o), s.undo1[t], bg);
+        l = fmaf(settle(l, p.s1, e, NT1, KT1, 2 * o + 1), s.undo1[t], bl);
+        if (p.has_limit) {
+          g = min_nan(g, p.limit);
+          l = max_nan(min_nan(l, p.limit), -p.limit);
+        }
+        const float sg = __fdividef(g, 1.0f + gemm_ex2(-p.alpha * g * 1.4426950408889634f)), v = fmaf(sg, l, sg);
+        if (live) __stcg(p.h + (int64_t)entry * p.ff + o, v);
+        top[q] = fmaxf(top[q], fabsf(v) < __int_as_float(0x7F800000) ? fabsf(v) : 0.0f);
+      }
+      if (m + 1 == n1 || nb == 0) {                           // the last of this expert's units here
+#pragma unroll
+        for (int q = 0; q < ROUNDS; ++q) {
+          if (q >= mine) break;
+#pragma unroll
+          for (int x = 8; x >= 1; x >>= 1) top[q] = fmaxf(top[q], __shfl_xor_sync(0xFFFFFFFFu, top[q], x));
+          const int r = r0 + q * STEP;
+          if (r < n && i == 0) {
+            const int t = s.who[e][r];
+            atomicMax(p.hmax + t * p.k + s.slot[e][t], __float_as_uint(top[q]));
+          }
+          top[q] = 0.0f;
+        }
+        bar_sync(2, MT_EPILOGUE);
+        if (tid == 0) {
+          __threadfence();
+          atomicAdd(p.done1 + e, min(was + 1, m + 1));
         }
       }
-      for (int64_t q = s_begin; q < s_end && ok; ++q) {
-        const int u = (int)(q / KS2), js = (int)(q - (int64_t)u * KS2), a = u / NB2, nb = u - a * NB2;
-        const int64_t tile = ((int64_t)s.act[a] * NT2 + (nb >> 2)) * KT2;
-        if (js < KS2 - 1) stage(&maps.v2, &maps.s2, MT_STAGE_KT, nb, tile + js * MT_STAGE_KT);
-        else stage(&maps.v2t, &maps.s2t, tail2, nb, tile + js * MT_STAGE_KT);
+    }
+    int have = -1, changes = -1;
+#pragma unroll 1
+    for (int m = n1; m < n1 + n2; ++m) {
+      const int u = first2 + m - n1, e = s.act[u / NB2], n = __popc(s.tokens[e]), lane_row = tid & 31;
+      if (e != have) { have = e; ++changes; }
+      mbar_wait_short(SUMS(m & 1), (m >> 1) & 1u, ctl, 1005);
+      for (int r = tid >> 5; r < n; r += MT_EPILOGUE / 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += s_red[m & 1][w][r * MT_RED_LD + lane_row];
+        if (two_terms(n, NBLK)) {
+#pragma unroll
+          for (int w = 0; w < 8; ++w) v += s_red[m & 1][w][(n + r) * MT_RED_LD + lane_row];
+        }
+        __stcg(p.part + ((int64_t)(u + c) * p.T + r) * MT_UNIT + lane_row, settle(v, p.s2, e, NT2, KT2, (u % NB2) * MT_UNIT + lane_row) * s.undo2[changes & 3][r]);
       }
-      if (!ok) {                                              // copies in flight land before the block's shared memory goes
-        const uint32_t lo = it > (uint32_t)p.stages ? it - p.stages : 0;
-        for (uint32_t j = lo; j < it; ++j)
-          for (uint32_t t = 0; t < (1u << 16) && !mbar_test(FULL(j % p.stages), (j / p.stages) & 1u); ++t) __nanosleep(64);
-      }
+      __syncwarp();
+      if ((tid & 31) == 0) mbar_arrive(TAKEN(m & 1));
+    }
+    bar_sync(2, MT_EPILOGUE);
+    for (int i = tid; i < n2; i += MT_EPILOGUE) {
+      const int u = first2 + i;
+      __threadfence();
+      atomicAdd(p.done2 + u % NB2, min(s_end, (u + 1) * KS2) - max(s_begin, u * KS2));
     }
     return;
   }
 
   // ================================= consumers =================================================================
-  const int wk = warp & 7, slab = warp >> 3, qrow = lane >> 2, c4 = lane & 3;
-  const int tid = threadIdx.x;
-  bool dead = false;                    // a wait ran out: the rest is gone through without waiting, its results are void
-  uint32_t it = 0, buf = 0;
+  const int wk = warp & 7, slab = warp >> 3, qrow = lane >> 2, c4 = lane & 3, tid = threadIdx.x;
+  // (where a wait runs out, this and the following ones return, the rest is gone through and its results are void)
+  int ri = 0;                           // place in the ring
+  uint32_t rp = 0;
   float acc[NBLK][4];
-
-  // staged token column col, eight k from 8 * k8 on
-  auto tok_at = [&](int col, int k8) { return toks + (uint32_t)((((k8 >> 2) * NBLK + (col >> 3)) * 8 + (col & 7)) * 64 + (k8 & 3) * 16); };
-  auto red_at = [&](int row, int col) {
-    return (((row >> 4) * NBLK + (col >> 3)) * 32 + (row & 7) * 4 + ((col & 7) >> 1)) * 4 + ((row >> 3) & 1) * 2 + (col & 1);
-  };
-  // one stage of a unit: groups wk and wk + 8 of its up to sixteen
-  auto multiply = [&](int tiles, int group0, uint32_t blocks) {
-    const int i = it % p.stages;
-    if (!dead) dead = !__all_sync(0xFFFFFFFFu, mbar_wait(FULL(i), (it / p.stages) & 1u, ctl, 1002));
-    const uint32_t st = ring + (uint32_t)(i * MT_STAGE_BYTES), row = (uint32_t)(slab * 16 + qrow);
+  // This warp's tile of a stage, 16 rows x 128 k, times the columns of NB blocks from `xt` on.  Every load goes ahead of the arithmetic: what bounds
+  // the loop is the number of instructions and the way of one warp through a stage.
+  const uint32_t my_w = ring + (uint32_t)(wk * 2048 + (slab * 16 + qrow) * 16 + c4 * 4), my_s = ring + (uint32_t)(MT_STAGE_VALUES + wk * 128 + (slab * 16 + qrow) * 4);
+  const uint32_t my_x = toks + (uint32_t)(wk * 4 * NBLK * 512 + qrow * 64 + c4 * 16);
+  auto multiply = [&](auto nb_tag, bool live, uint32_t xt) {
+    constexpr int NB = decltype(nb_tag)::value;
+    mbar_wait_short(FULL(ri), rp, ctl, 1002);
+    if (live) {
+      const uint32_t wt = my_w + (uint32_t)(ri * MT_STAGE_BYTES), sc = my_s + (uint32_t)(ri * MT_STAGE_BYTES);
+      const uint32_t sl = lds32(sc), sh = lds32(sc + 32);
+      uint32_t wl[4], wh[4];
+      uint4 xb[4][NB];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int g = wk + 8 * hf;
-      if (g < tiles * 4) {
-        const uint32_t wl = lds32(st + g * 512 + row * 16 + c4 * 4), wh = lds32(st + g * 512 + row * 16 + 128 + c4 * 4);
-        const uint32_t sc = st + MT_STAGE_VALUES + (g >> 2) * 128 + row * 4 + (g & 3);
-        const float fl = e8m0_f32(lds8(sc)), fh = e8m0_f32(lds8(sc + 32));
+      for (int g = 0; g < 4; ++g) {
+        wl[g] = lds32(wt + g * 512);
+        wh[g] = lds32(wt + g * 512 + 128);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) xb[g][b] = lds128(xt + (uint32_t)((g * NBLK + b) * 512));
+      }
+      float fl[4], fh[4];
+      e8m0_word(sl, fl);
+      e8m0_word(sh, fh);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
         uint32_t lo[4], hi[4];
-        e2m1_word(wl, lo);
-        e2m1_word(wh, hi);
+        e2m1_word(wl[g], lo);
+        e2m1_word(wh[g], hi);
 #pragma unroll
-        for (int b = 0; b < NBLK; ++b)
-          if (NBLK == 1 || (blocks >> b & 1)) {
-            const uint4 xb = lds128(toks + (uint32_t)((((group0 + g) * NBLK + b) * 8 + qrow) * 64 + c4 * 16));
-            float dd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16(dd, lo[0], hi[0], lo[1], hi[1], xb.x, xb.y);
-            mma_f16(dd, lo[2], hi[2], lo[3], hi[3], xb.z, xb.w);
-            acc[b][0] = fmaf(fl, dd[0], acc[b][0]);
-            acc[b][1] = fmaf(fl, dd[1], acc[b][1]);
-            acc[b][2] = fmaf(fh, dd[2], acc[b][2]);
-            acc[b][3] = fmaf(fh, dd[3], acc[b][3]);
-          }
+        for (int b = 0; b < NB; ++b) {
+          float dd[4];
+          mma_f16_zero(dd, lo[0], hi[0], lo[1], hi[1], xb[g][b].x, xb[g][b].y);
+          mma_f16(dd, lo[2], hi[2], lo[3], hi[3], xb[g][b].z, xb[g][b].w);
+          acc[b][0] = fmaf(fl[g], dd[0], acc[b][0]);
+          acc[b][1] = fmaf(fl[g], dd[1], acc[b][1]);
+          acc[b][2] = fmaf(fh[g], dd[2], acc[b][2]);
+          acc[b][3] = fmaf(fh[g], dd[3], acc[b][3]);
+        }
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(EMPTY(i));
-    ++it;
+    if (lane == 0) mbar_arrive(EMPTY(ri));
+    if (++ri == p.stages) { ri = 0; rp ^= 1u; }
   };
-  auto clear = [&]() {
+
+  if (NBLK == 2) {
+    if (warp < p.T) stage_x(p, s, NBLK, toks, warp);
+    bar_sync(1, MT_CONSUMERS);
+  }
+  // ---- all units, fc1's and fc2's ----
+  int have = -1, changes = -1;          // expert whose rows of fc2 are staged
+  int first = 0, n_blocks = 1;          // blocks of columns that the expert's tokens are in
+  int place = u_begin / NB1, rest = u_begin - place * NB1;   // the unit's expert in the list of active ones, its place among the expert's units
+#pragma unroll 1
+  for (int m = 0; m < n1 + n2; ++m, ++rest) {
+    const bool one = m < n1;
+    if (m == n1) { place = first2 / NB2; rest = first2 - place * NB2; }
+    if (rest == (one ? NB1 : NB2)) { rest = 0; ++place; }
+    const int e = s.act[place], KT = one ? KT1 : KT2;
+    const int js0 = m == n1 ? s_begin - first2 * KS2 : 0, js1 = one ? KS1 : m + 1 == n1 + n2 ? s_end - (first2 + n2 - 1) * KS2 : KS2;
+    const uint32_t mask = s.tokens[e];
+    if (one) {
+      first = mask & 0xFFu ? 0 : 1;
+      n_blocks = NBLK == 2 && !first && mask >> 8 ? 2 : 1;
+    } else if (e != have) {
+      if (tid == 0) wait_count(p.done1 + e, NB1, ctl, 1003);
+      bar_sync(1, MT_CONSUMERS);                              // fc1's rows are there, and the staged ones have been read
+      const int n = __popc(mask);
+      ++changes;
+      stage_h(p, s, NBLK, toks, e, n, KT2, changes & 3, warp);
+      bar_sync(1, MT_CONSUMERS);
+      have = e;
+      first = 0;
+      n_blocks = (two_terms(n, NBLK) ? 2 * n : n) > 8 ? 2 : 1;
+    }
 #pragma unroll
     for (int b = 0; b < NBLK; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[b][j] = 0.0f;
-  };
-  // the eight shares of k meet; the buffers alternate, so that a warp may be a unit ahead of those that still add
-  auto meet = [&]() {
-    buf ^= 1u;
+    uint32_t xt = my_x + (uint32_t)(js0 * MT_STAGE_KT * 4 * NBLK * 512);
+    if (NBLK == 1 || n_blocks == 1) {
+      xt += (uint32_t)(first * 512);
+#pragma unroll 1
+      for (int js = js0; js < js1; ++js, xt += MT_STAGE_KT * 4 * NBLK * 512)
+        multiply(std::integral_constant<int, 1>(), js * MT_STAGE_KT + wk < KT, xt);
+    } else {
+#pragma unroll 1
+      for (int js = js0; js < js1; ++js, xt += MT_STAGE_KT * 4 * NBLK * 512)
+        multiply(std::integral_constant<int, NBLK>(), js * MT_STAGE_KT + wk < KT, xt);
+    }
+    // the warp's share of the unit's sums goes to the epilogue; two buffers
+    if (m >= 2) mbar_wait_short(TAKEN(m & 1), ((m >> 1) & 1u) ^ 1u, ctl, 1006);
 #pragma unroll
     for (int b = 0; b < NBLK; ++b)
-      *reinterpret_cast<float4*>(&s_red[buf][wk][((slab * NBLK + b) * 32 + lane) * 4]) = make_float4(acc[b][0], acc[b][1], acc[b][2], acc[b][3]);
-    consumer_bar();
-  };
-  auto summed = [&](int row, int col) {
-    const int at = red_at(row, col);
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) v += s_red[buf][w][at];
-    return v;
-  };
-
-  // ---- tokens as the columns of fc1, in their order ----
-  for (int i = tid; i < p.T * KT1 * 16; i += MT_CONSUMERS) {
-    const int t = i / (KT1 * 16), k8 = i - t * (KT1 * 16);
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    if (k8 * 8 < p.d) {
-      if (p.x_dtype == MOE_F16) load8((const __half*)p.x + t * p.ld_x + k8 * 8, v);
-      else load8((const __nv_bfloat16*)p.x + t * p.ld_x + k8 * 8, v);
-    }
-    const float down = pow2(-row_exponent(__ldcg(p.xmax + t)));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= down;
-    sts128(tok_at(t, k8), pack8(v));
-  }
-  if (tid < p.T) s.undo[tid] = pow2(row_exponent(__ldcg(p.xmax + tid)));
-  consumer_bar();
-
-  // ---- fc1 ----
-  for (int u = u_begin; u < u_end; ++u) {
-    const int a = u / NB1, nb = u - a * NB1, e = s.act[a];
-    const uint32_t mask = s.tokens[e];
-    const uint32_t blocks = (mask & 0xFFu ? 1u : 0u) | (mask >> 8 ? 2u : 0u);
-    clear();
-    for (int js = 0; js < KS1; ++js) multiply(min(MT_STAGE_KT, KT1 - js * MT_STAGE_KT), js * 16, blocks);
-    meet();
-    const int n = __popc(mask);
-    if ((tid & ~31) < n * 16) {                               // sixteen outputs of a token by half a warp
-      const bool live = tid < n * 16;
-      const int t = __fns(mask, 0, live ? (tid >> 4) + 1 : n), i = tid & 15, o = nb * 16 + i;
-      float g = summed(2 * i, t) * s.undo[t], l = summed(2 * i + 1, t) * s.undo[t];
-      if (p.b1) {
-        g += load_bias(p.b1, p.b1_dtype, e * p.ld_b1 + 2 * o);
-        l += load_bias(p.b1, p.b1_dtype, e * p.ld_b1 + 2 * o + 1);
+      if (b < n_blocks) {
+        float* at = &s_red[m & 1][wk][((first + b) * 8 + c4 * 2) * MT_RED_LD + slab * 16 + qrow];
+        at[0] = acc[b][0];
+        at[MT_RED_LD] = acc[b][1];
+        at[8] = acc[b][2];
+        at[MT_RED_LD + 8] = acc[b][3];
       }
-      if (p.has_limit) {
-        g = min_nan(g, p.limit);
-        l = max_nan(min_nan(l, p.limit), -p.limit);
-      }
-      const float sg = __fdividef(g, 1.0f + gemm_ex2(-p.alpha * g * 1.4426950408889634f)), v = fmaf(sg, l, sg);
-      const int entry = t * p.k + s.slot[e][t];
-      if (live) __stcg(p.h + (int64_t)entry * p.ff + o, v);
-      float m = fabsf(v) < __int_as_float(0x7F800000) ? fabsf(v) : 0.0f;
-#pragma unroll
-      for (int x = 8; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-      if (live && i == 0) atomicMax(p.hmax + entry, __float_as_uint(m));
-    }
-    if (u + 1 == u_end || nb + 1 == NB1) {                    // the last of this expert's units here
-      consumer_bar();
-      if (tid == 0) {
-        __threadfence();
-        atomicAdd(p.done1 + e, min(nb + 1, u + 1 - u_begin));
-      }
-    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(SUMS(m & 1));
   }
 
-  // ---- fc2 ----
-  int have = -1, n = 0, cols = 0;       // expert whose rows are staged, its tokens, columns they take
-  for (int64_t q = s_begin; q < s_end;) {
-    const int u = (int)(q / KS2), js0 = (int)(q - (int64_t)u * KS2), a = u / NB2, e = s.act[a];
-    const int js1 = (int)min((int64_t)KS2, js0 + (s_end - q));
-    const uint32_t mask = s.tokens[e];
-    if (e != have) {
-      if (tid == 0 && !dead) {
-        const long long t0 = clock64();
-        while (ld_acquire(p.done1 + e) < NB1) {
-          if (s.abort) break;
-          if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
-            s.abort = 1;
-            if (p.status) atomicExch(p.status, 1003);
-            break;
-          }
-        }
-      }
-      consumer_bar();                                         // fc1's rows are there, and the staged ones have been read
-      n = __popc(mask);
-      const bool two = 2 * n <= 8 * NBLK;
-      cols = two ? 2 * n : n;
-      for (int i = tid; i < n * KT2 * 16; i += MT_CONSUMERS) {
-        const int r = i / (KT2 * 16), k8 = i - r * (KT2 * 16), t = __fns(mask, 0, r + 1), entry = t * p.k + s.slot[e][t];
-        const float down = pow2(-row_exponent(__uint_as_float(__ldcg(p.hmax + entry))));
-        float v[8], w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        if (k8 * 8 < p.ff) {
-          const float4* src = reinterpret_cast<const float4*>(p.h + (int64_t)entry * p.ff + k8 * 8);
-          const float4 v0 = __ldcg(src), v1 = __ldcg(src + 1);
-          v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w; v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] *= down;
-          const float left = v[j] - __half2float(__float2half_rn(v[j]));
-          w[j] = isfinite(left) ? left : 0.0f;                // (infinities and NaN are the first term's)
-        }
-        sts128(tok_at(r, k8), pack8(v));
-        if (two) sts128(tok_at(n + r, k8), pack8(w));
-      }
-      if (tid < n) {
-        const int t = __fns(mask, 0, tid + 1);
-        s.undo[tid] = pow2(row_exponent(__uint_as_float(__ldcg(p.hmax + t * p.k + s.slot[e][t]))));
-      }
-      consumer_bar();
-      have = e;
-    }
-    clear();
-    for (int js = js0; js < js1; ++js) multiply(min(MT_STAGE_KT, KT2 - js * MT_STAGE_KT), js * 16, cols > 8 ? 3u : 1u);
-    meet();
-    if (tid < n * MT_UNIT) {
-      const int r = tid >> 5;
-      float v = summed(lane, r);
-      if (cols > n) v += summed(lane, n + r);
-      __stcg(p.part + ((int64_t)(u + c) * p.T + r) * MT_UNIT + lane, v * s.undo[r]);
-    }
-    q += js1 - js0;
-  }
-
-  // ---- whoever completes 32 output columns adds them up ----
-  consumer_bar();
-  const int first = (int)(s_begin / KS2), n_parts = s_end > s_begin ? (int)((s_end - 1) / KS2) - first + 1 : 0;
-  for (int i = tid; i < n_parts; i += MT_CONSUMERS) {
-    const int u = first + i, nb = u % NB2;
-    const int mine = (int)(min(s_end, (int64_t)(u + 1) * KS2) - max(s_begin, (int64_t)u * KS2));
-    __threadfence();
-    if (atomicAdd(p.done2 + nb, mine) + mine == A * KS2) s.done[atomicAdd(&s.n_done, 1)] = nb;
-  }
-  consumer_bar();
-  const int n_done = s.n_done;
-  if (n_done == 0) return;
-  __threadfence();
-  for (int i = tid; i < n_done * p.T * MT_UNIT; i += MT_CONSUMERS) {
-    const int w = i >> 5, nb = s.done[w / p.T], t = w % p.T, o = nb * MT_UNIT + lane;
+  // ---- the selected experts' sums meet: a warp takes 32 outputs of a token as soon as all of their stages are done ----
+  for (int i = warp * G + c; i < NB2 * p.T; i += MT_WARPS * G) {
+    const int t = i / NB2, nb = i - t * NB2, o = nb * MT_UNIT + lane;
     float y = 0.0f;
-    for (int j = 0; j < p.k; ++j) {
-      const int e = s.sel[t][j], u = (int)s.rank[e] * NB2 + nb, r = __popc(s.tokens[e] & ((1u << t) - 1u));
-      // the CTAs whose ranges the unit's stages are in (those between with nothing to do where there are fewer stages than CTAs)
-      const int c0 = (int)((((int64_t)u * KS2 + 1) * G - 1) / S2), c1 = (int)((((int64_t)(u + 1) * KS2) * G - 1) / S2);
-      float v = p.b2 ? load_bias(p.b2, p.b2_dtype, e * p.ld_b2 + o) : 0.0f;
-      for (int cc = c0; cc <= c1; ++cc)
-        if (S2 * cc / G < S2 * (cc + 1) / G) v += __ldcg(p.part + ((int64_t)(u + cc) * p.T + r) * MT_UNIT + lane);
-      y = fmaf(s.gate[t][j], v, y);
+    for (int j0 = 0; j0 < p.k; j0 += 4) {
+      float v[4], b[4];
+      int c0[4], c1[4];
+      const float* part[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        b[x] = 0.0f;
+        c0[x] = c1[x] = 0;
+        part[x] = nullptr;
+        if (j0 + x < p.k) {
+          const int e = s.sel[t][j0 + x], u = (int)s.rank[e] * NB2 + nb, r = __popc(s.tokens[e] & ((1u << t) - 1u));
+          // the CTAs whose ranges the unit's stages are in (those between with nothing to do where there are fewer stages than CTAs)
+          c0[x] = ((u * KS2 + 1) * G - 1) / S2;
+          c1[x] = ((u + 1) * KS2 * G - 1) / S2;
+          part[x] = p.part + ((int64_t)u * p.T + r) * MT_UNIT + lane;
+          if (p.b2) b[x] = load_bias(p.b2, p.b2_dtype, e * p.ld_b2 + o);
+        }
+      }
+      wait_count(p.done2 + nb, A * KS2, ctl, 1004);
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[x] = j0 + x < p.k ? __ldcg(part[x] + (int64_t)c0[x] * p.T * MT_UNIT) : 0.0f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (j0 + x >= p.k) break;
+        for (int cc = c0[x] + 1; cc <= c1[x]; ++cc)
+          if (S2 * cc / G < S2 * (cc + 1) / G) v[x] += __ldcg(part[x] + (int64_t)cc * p.T * MT_UNIT);
+        y = fmaf(s.gate[t][j0 + x], v[x] + b[x], y);
+      }
     }
     if (p.y_dtype == MOE_F16) ((__half*)p.y)[t * p.ld_y + o] = __float2half_rn(y);
     else ((__nv_bfloat16*)p.y)[t * p.ld_y + o] = __float2bfloat16_rn(y);
@@ -666,6 +850,7 @@ extern "C" __attribute__((visibility("default"))) int moe_layer_tokens(const Moe
   TokensParams p = {};
   p.x = a.x; p.x_dtype = a.x_dtype; p.ld_x = a.ld_x;
   p.T = a.T; p.d = a.d; p.ff = a.ff; p.E = a.E; p.k = a.k;
+  p.s1 = (const uint8_t*)a.w1_scale; p.s2 = (const uint8_t*)a.w2_scale;
   p.b1 = a.b1; p.b1_dtype = a.b1_dtype; p.ld_b1 = a.ld_b1;
   p.b2 = a.b2; p.b2_dtype = a.b2_dtype; p.ld_b2 = a.ld_b2;
   p.alpha = a.act_alpha; p.limit = a.act_limit; p.has_limit = a.act_has_limit;

@@ -128,7 +128,8 @@ _STATUS_TEXT = {
     803: "router kernel: the MMA warp waited for a free accumulator", 804: "router kernel: the selection waited for the accumulator",
     901: "expert-parallel peer barrier: a rank did not arrive within the limit; the step after it read stale peer buffers",
     1001: "layer of a few tokens: the weight producer waited for a free stage", 1002: "layer of a few tokens: a warp waited for weights",
-    1003: "layer of a few tokens: fc2 waited for fc1's rows",
+    1003: "layer of a few tokens: fc2 waited for fc1's rows", 1004: "layer of a few tokens: the combine waited for fc2's sums",
+    1005: "layer of a few tokens: the epilogue waited for a unit's sums", 1006: "layer of a few tokens: a warp waited for a free buffer of sums",
 }
 
 
