@@ -378,6 +378,33 @@ typedef struct {
 size_t moe_layer_tokens_workspace_bytes(const MoeTokensArgs* args);
 int moe_layer_tokens(const MoeTokensArgs* args, void* stream);
 
+/* ---- a shared projection with low-rank adapters of many requests ---------------------------------
+ * y_t = x_t W + bias + scale[a] (x_t A_a) B_a with a = indx[t]; an index that is no adapter (negative, or >= n_adapters) leaves the second part out.
+ * x [T, K], y [T, N], w_t (W transposed, [N, K]) and the adapters in one 16-bit type (dtype: bf16 or fp16), sums in fp32, y rounded once.  An adapter's ranks,
+ * padded with zeros to a multiple of 16, are pieces of 16: `first` [n_adapters + 1] (device) numbers them through, max_pieces is the largest count
+ * of one adapter.  `a`: the pieces' 16 rows of K each, pitch ld_a >= K rounded up to 8, zeros past K.  `b`: per piece [N rounded up to 128 / 8][2][8][8]:
+ * value [g][h][r][c] is B's rank 8 h + c at output 8 g + r, zero past N; finite (the product of a block of tokens multiplies other
+ * adapters' B by zero).  x, w_t, a: 16-byte aligned rows, x's padded to 8 values (of any finite contents past K where adapters are given).
+ * bias (fp32, fp16 or bf16) and, with n_adapters = 0, everything of the adapters may be NULL.  workspace: 256-byte aligned,
+ * moe_lora_matmul_workspace_bytes(args) bytes of any contents; calls that may overlap need one each.  Two kernels (one without adapters);
+ * bounded waits (status codes 11xx). */
+typedef struct {
+  const void* x; int dtype; int64_t ld_x; int64_t T; int K, N;
+  const void* w_t; int64_t ld_w;
+  const void* bias; int bias_dtype;
+  int n_adapters, max_pieces;
+  const void* a; int64_t ld_a;
+  const void* b;
+  const int32_t* first;
+  const float* scale;
+  const int32_t* indx;
+  void* y; int64_t ld_y;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;
+} MoeLoraArgs;
+size_t moe_lora_matmul_workspace_bytes(const MoeLoraArgs* args);
+int moe_lora_matmul(const MoeLoraArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ from .tensor import (FP4, BitmatrixMetadata, RaggedTensorMetadata, SparseMatrix,
                      convert_layout, make_bitmatrix_metadata, make_ragged_tensor_metadata,
                      remap_ragged_tensor_metadata, wrap_torch_tensor)
 from .topk import topk  # noqa: F401
+from .lora import LoraAdapters, matmul_lora, prepare_lora_adapters, prepare_projection_weight  # noqa: F401
 from .moe_tokens import moe_layer_tokens  # noqa: F401
 from .weights_io import from_block_checkpoint, load_layer_weights, save_layer_weights  # noqa: F401
 from .distributed import (ExptAssignment, Mesh, SymmetricMemoryPool, convert_dp_to_ep, convert_ep_to_dp,  # noqa: F401

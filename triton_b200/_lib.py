@@ -86,6 +86,8 @@ PROTOTYPES = {
     "moe_gather_reduce_rows": (i32, [vp, i64, vp, i64, i32, i64, vp, i64, vp]),
     "moe_layer_tokens_workspace_bytes": (sz, [vp]),
     "moe_layer_tokens": (i32, [vp, vp]),
+    "moe_lora_matmul_workspace_bytes": (sz, [vp]),
+    "moe_lora_matmul": (i32, [vp, vp]),
     "moe_scatter_rows": (i32, [vp, i64, vp, i64, i64, vp, i64, vp]),
 }
 

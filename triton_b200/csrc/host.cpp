@@ -20,7 +20,8 @@ struct Lib {
   X(moe_last_error) X(moe_route) X(moe_route_positions) X(moe_route_workspace) X(moe_grouped_gemm) X(moe_gemm_mx_workspace_bytes) \
   X(moe_reduce) X(moe_downcast_mxfp4) X(moe_upcast_mxfp4) X(moe_bitmatrix_metadata) X(moe_bitmatrix_metadata_workspace) \
   X(moe_router_topk) X(moe_copy2) X(moe_step_graph_create) X(moe_step_graph_launch) X(moe_step_graph_destroy) \
-  X(moe_gemm_kernel_name) X(moe_grouped_gemm_chain) X(moe_layer_tokens) X(moe_layer_tokens_workspace_bytes)
+  X(moe_gemm_kernel_name) X(moe_grouped_gemm_chain) X(moe_layer_tokens) X(moe_layer_tokens_workspace_bytes) \
+  X(moe_lora_matmul) X(moe_lora_matmul_workspace_bytes)
 #define X(name) decltype(&::name) name = nullptr;
   MOE_HOST_FUNCTIONS(X)
 #undef X
@@ -375,6 +376,49 @@ Tensor moe_tokens(const Tensor& x_, const Tensor& wg, const OptTensor& bg, int64
   return y;
 }
 
+// ---- a shared projection with low-rank adapters --------------------------------------------------------------------
+// w in the kernel's memory order; adapters: (a, b, first, scale, adapters, most pieces of one) or None, then indx too
+Tensor lora(const Tensor& x_, const Tensor& w, const OptTensor& bias, const py::object& adapters, const OptTensor& indx_, const Tensor& status) {
+  need_cuda(x_);
+  const c10::cuda::CUDAGuard guard(x_.device());
+  const int64_t T = x_.size(0), K = x_.size(1), N = w.size(1), K8 = cdiv(K, 8) * 8;
+  same_device(x_, w, "w");
+  same_device(x_, status, "the status word");
+  Tensor x = x_;
+  if (K8 != K) {                         // rows end with zeros
+    x = empty({T, K8}, x_.scalar_type(), x_);
+    x.narrow(1, 0, K).copy_(x_);
+    x.narrow(1, K, K8 - K).zero_();
+  } else {
+    x = aligned_rows(x_);
+  }
+  MoeLoraArgs g{};
+  g.x = x.data_ptr(); g.dtype = dtype_code(x); g.ld_x = T > 1 ? x.stride(0) : K8; g.T = T; g.K = (int)K; g.N = (int)N;
+  g.w_t = w.data_ptr(); g.ld_w = N > 1 ? w.stride(1) : K8;
+  if (bias) { same_device(x, *bias, "bias"); g.bias = bias->data_ptr(); g.bias_dtype = dtype_code(*bias); }
+  Tensor a, b, first, scale, indx;
+  if (!adapters.is_none()) {
+    const py::tuple t = adapters;
+    a = t[0].cast<Tensor>(); b = t[1].cast<Tensor>(); first = t[2].cast<Tensor>(); scale = t[3].cast<Tensor>();
+    indx = indx_->scalar_type() == at::kInt ? indx_->contiguous() : indx_->clamp(-1, INT32_MAX).to(at::kInt).contiguous();
+    for (const Tensor* q : {&a, &b, &first, &scale, &indx}) same_device(x, *q, "an adapter or the index");
+    g.a = a.data_ptr(); g.ld_a = a.size(1); g.b = b.data_ptr(); g.first = first.data_ptr<int32_t>(); g.scale = scale.data_ptr<float>();
+    g.n_adapters = t[4].cast<int>(); g.max_pieces = t[5].cast<int>();
+    g.indx = indx.data_ptr<int32_t>();
+  }
+  Tensor y = empty({T, N}, x.scalar_type(), x), ws;
+  if (y.numel() == 0) return y;
+  g.y = y.data_ptr(); g.ld_y = N;
+  g.workspace_bytes = lib.moe_lora_matmul_workspace_bytes(&g);
+  if (g.workspace_bytes > 0) {
+    ws = empty({(int64_t)g.workspace_bytes}, at::kByte, x);
+    g.workspace = ws.data_ptr();
+  }
+  g.status = status.data_ptr<int32_t>();
+  check(lib.moe_lora_matmul(&g, stream()), "moe_lora_matmul");
+  return y;
+}
+
 // ---- quantiser, combine --------------------------------------------------------------------------------------------
 // [batch, outer, quant] element strides of `t` with its last axis quantised; false when the leading axes do not merge into two
 bool collapse3(const Tensor& t, int64_t (&e)[2], int64_t (&s)[2]) {
@@ -541,6 +585,7 @@ PYBIND11_MODULE(_host, m) {
         py::arg("y_dtype"), py::arg("tuning"), py::arg("rows_per_expert") = 0, py::arg("swiglu") = false);
   m.def("layer", &layer);
   m.def("moe_tokens", &moe_tokens);
+  m.def("lora", &lora);
   m.def("downcast", &downcast);
   m.def("upcast", &upcast);
   m.def("reduce", &reduce);

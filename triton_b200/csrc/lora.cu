@@ -1,0 +1,541 @@
+// A projection that all requests share, with each request's own low-rank adapter beside it:
+//     y_t = x_t W + bias + s_a (x_t A_a) B_a,   a = indx[t]; no second part where indx[t] is no adapter.
+//
+// An adapter's ranks go in pieces of 16, so adapters of different ranks lie behind one another: A as rows of K, B as tiles in the order the tensor core
+// takes them (lora_adapters layout in the header).  Two kernels:
+//  1. lora_shrink_kernel: t = s_a x A_a for every token, fp32, into the workspace.  A piece of an adapter (16 rows of A) times 8 or 64 tokens is what a CTA
+//     has, on mma.sync with operands straight from global memory: there are 16 ranks, too few for a tcgen05 operand of 128 rows, and at single
+//     tokens reading A is all there is to do.
+//  2. the product: W's tiles and x's through a ring by TMA, tcgen05.mma.kind::f16 into fp32 in tensor memory; then, into the same accumulator, one MMA per
+//     piece and term: B's tile times the tokens' t, zero for the tokens of other adapters, so that a block of tokens may hold any mixture.  t enters in two
+//     terms (hi + lo, 16 bits of it in bf16), so it costs the result nothing.
+// The second has two forms: lora_stream_kernel for few tokens (weight rows are the MMA's 128 rows, up to 256 tokens its columns, K cut over a cluster) and
+// lora_pair_kernel for many (a pair of SMs per tile of 256 tokens x 256 outputs).
+#include "gemm_tc_common.cuh"
+#include <cuda_fp16.h>
+#include <type_traits>
+
+namespace {
+
+constexpr int LR_PIECE = 16;                   // ranks of a piece
+constexpr int LR_TILE_N = 128;                 // outputs of a weight tile
+constexpr int LR_PIECE_BYTES = LR_TILE_N * LR_PIECE * 2;
+
+struct LoraParams {
+  const void* x; int64_t ld_x; int T, K, N, NP;        // NP: outputs rounded up to 128, rows of a piece of B
+  const void* bias; int bias_dtype;
+  const void* a; int64_t ld_a;
+  const uint8_t* b;
+  const int32_t* first; const float* scale; int n_adapters, max_pieces;
+  const int32_t* indx;
+  float* t; int64_t ld_t; int t_parts; int64_t t_part_stride;     // shares of k whose sums make up t
+  void* y; int64_t ld_y;
+  int32_t* status;
+};
+
+// ---- shrink ----------------------------------------------------------------------------------------------------
+template <typename T16> __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T16) == 2 && std::is_same<T16, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Adapter of each of `rows` tokens from row0 on (-1: none, and for the rows past them) and the list of those that occur, in the order of their first
+// token.  All threads of the block call; `idx` and `list` are in shared memory; behind a barrier, with one at the end.
+__device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, int rows, int block_rows, int* idx, int* list, int* count) {
+  for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {
+    const int a = r < rows && p.indx ? p.indx[row0 + r] : -1;
+    idx[r] = a >= 0 && a < p.n_adapters ? a : -1;
+  }
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  for (int r0 = 0; r0 < block_rows; r0 += 32) {             // one warp, 32 tokens at a time
+    if (threadIdx.x >= 32) break;
+    const int r = r0 + threadIdx.x, a = r < block_rows ? idx[r] : -1;
+    bool fresh = a >= 0;
+    const int n = *count;
+    for (int i = 0; i < n && fresh; ++i) fresh = list[i] != a;
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, a);
+    fresh = fresh && (int)threadIdx.x == __ffs(same) - 1;
+    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, fresh);
+    __syncwarp();
+    if (fresh) list[n + __popc(mask & ((1u << threadIdx.x) - 1u))] = a;
+    __syncwarp();
+    if (threadIdx.x == 0) *count = n + __popc(mask);
+    __syncwarp();
+  }
+  __syncthreads();
+}
+
+constexpr int SH_WARPS = 8;
+
+// grid: (blocks of 8 NB tokens, pieces of an adapter, shares of k x list places)
+template <typename T16, int NB>
+__global__ void __launch_bounds__(SH_WARPS * 32) lora_shrink_kernel(const LoraParams p, const int places) {
+  __shared__ int s_idx[8 * NB], s_list[8 * NB], s_count;
+  __shared__ float s_sum[SH_WARPS][NB][32][4];
+  pdl_begin();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qrow = lane >> 2, c4 = lane & 3;
+  const int64_t row0 = (int64_t)blockIdx.x * (8 * NB);
+  const int rows = (int)min((int64_t)(8 * NB), (int64_t)p.T - row0);
+  const int place = blockIdx.z % places, part = blockIdx.z / places;
+  adapters_of(p, row0, rows, 8 * NB, s_idx, s_list, &s_count);
+  const int K8 = (p.K + 7) & ~7, blocks = (K8 + 31) >> 5, b0 = blocks * part / p.t_parts, b1 = blocks * (part + 1) / p.t_parts;
+  for (int l = place; l < s_count; l += places) {
+    const int a = s_list[l], f = p.first[a];
+    if ((int)blockIdx.y >= p.first[a + 1] - f) continue;      // (uniform)
+    const T16* ra = (const T16*)p.a + (int64_t)(f + blockIdx.y) * LR_PIECE * p.ld_a;
+    float acc[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
+    constexpr int UNROLL = NB == 1 ? 4 : 2;
+    for (int b = b0 + warp; b < b1; b += UNROLL * SH_WARPS) {
+      uint4 lo[UNROLL], hi[UNROLL], xv[UNROLL][NB];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int k = (b + u * SH_WARPS) * 32 + c4 * 8;       // a lane's eight consecutive k are its places in two MMAs
+        const bool in = b + u * SH_WARPS < b1 && k < K8;
+        lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+        if (in) {
+          lo[u] = *reinterpret_cast<const uint4*>(ra + qrow * p.ld_a + k);
+          hi[u] = *reinterpret_cast<const uint4*>(ra + (qrow + 8) * p.ld_a + k);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          xv[u][n] = make_uint4(0, 0, 0, 0);
+          if (in && n * 8 + qrow < rows) xv[u][n] = *reinterpret_cast<const uint4*>((const T16*)p.x + (row0 + n * 8 + qrow) * p.ld_x + k);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          mma_16816<T16>(acc[n], lo[u].x, hi[u].x, lo[u].y, hi[u].y, xv[u][n].x, xv[u][n].y);
+          mma_16816<T16>(acc[n], lo[u].z, hi[u].z, lo[u].w, hi[u].w, xv[u][n].z, xv[u][n].w);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s_sum[warp][n][lane][j] = acc[n][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < NB * 128; i += SH_WARPS * 32) {
+      const int n = i >> 7, token = n * 8 + ((i >> 4) & 7), rank = i & 15;       // accumulator: rank rows, token columns
+      const int ln = (rank & 7) * 4 + ((token & 7) >> 1), j = (rank >> 3) * 2 + (token & 1);
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < SH_WARPS; ++w) v += s_sum[w][n][ln][j];
+      if (s_idx[token] == a)
+        p.t[part * p.t_part_stride + (row0 + token) * p.ld_t + blockIdx.y * LR_PIECE + rank] = v * p.scale[a];
+    }
+    __syncthreads();
+  }
+}
+
+// ---- pieces as MMA operands --------------------------------------------------------------------------------------
+// Operands of 16 k without swizzle: eight rows of 16 bytes are 128 bytes in a row, the two halves of k follow one another, then the next eight rows.
+constexpr uint32_t PIECE_DESC_LO = (128u >> 4) << 16;                   // leading byte offset: between the halves of k
+// (An address of a CTA in a cluster has its rank from bit 24 on, which in a descriptor would be part of the leading byte offset.)
+__device__ __forceinline__ uint32_t piece_desc(uint32_t at) { return PIECE_DESC_LO | ((at & 0x3FFFFu) >> 4); }
+constexpr uint32_t PIECE_DESC_HI = (256u >> 4) | (1u << 14);            // stride byte offset: between groups of eight rows; sm_100, no swizzle
+__device__ __forceinline__ uint32_t lr_idesc(bool f16, int m, int n) {
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void elect_mma_piece(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PIECE_DESC_HI)
+      : "memory");
+}
+template <typename T16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  T16 h[2] = {from_f32<T16>(a), from_f32<T16>(b)};
+  return *reinterpret_cast<const uint32_t*>(h);
+}
+// Sixteen ranks of token row `row` (of the block; `live`: it has this adapter) as row `at` of the operand: high terms at dst, what they leave at dst + lo
+template <typename T16>
+__device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, int64_t token, int rank0, uint32_t dst, uint32_t lo, int at) {
+  uint4 h[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, l[2] = {h[0], h[0]};
+  if (live) {
+    float v[16];
+    const float4* src = reinterpret_cast<const float4*>(p.t + token * p.ld_t + rank0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 q = src[i];
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    }
+    for (int s = 1; s < p.t_parts; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 q = *(reinterpret_cast<const float4*>(p.t + s * p.t_part_stride + token * p.ld_t + rank0) + i);
+        v[4 * i] += q.x; v[4 * i + 1] += q.y; v[4 * i + 2] += q.z; v[4 * i + 3] += q.w;
+      }
+    float left[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float d = v[i] - to_f32<T16>(from_f32<T16>(v[i]));
+      left[i] = isfinite(d) ? d : 0.0f;                       // infinities and NaN are the first term's
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      h[i] = make_uint4(pack2<T16>(v[8 * i], v[8 * i + 1]), pack2<T16>(v[8 * i + 2], v[8 * i + 3]), pack2<T16>(v[8 * i + 4], v[8 * i + 5]), pack2<T16>(v[8 * i + 6], v[8 * i + 7]));
+      l[i] = make_uint4(pack2<T16>(left[8 * i], left[8 * i + 1]), pack2<T16>(left[8 * i + 2], left[8 * i + 3]), pack2<T16>(left[8 * i + 4], left[8 * i + 5]), pack2<T16>(left[8 * i + 6], left[8 * i + 7]));
+    }
+  }
+  const uint32_t to = dst + (uint32_t)((at >> 3) * 256 + (at & 7) * 16);
+  sts128(to, h[0]);
+  sts128(to + 128, h[1]);
+  sts128(to + lo, l[0]);
+  sts128(to + lo + 128, l[1]);
+}
+
+// ---- few tokens ------------------------------------------------------------------------------------------------
+constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-5 epilogue, 6-9 write the tokens' side of the pieces
+constexpr int LS_MAX_STAGES = 8, LS_MAX_PIECES = 4, LS_MAX_TB = 256;
+
+struct StreamPlan { int tb, splits, stages, pieces, smem; };      // tokens of a block, cluster, ring of k steps, ring of pieces, bytes
+
+template <typename T16>
+__global__ void __launch_bounds__(LS_THREADS, 2)
+lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem);
+  __shared__ __align__(8) uint64_t bars[2 * LS_MAX_STAGES + 2 * LS_MAX_PIECES + 1];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_count;
+  __shared__ int s_idx[LS_MAX_TB], s_list[LS_MAX_TB], s_first[LS_MAX_TB], s_np[LS_MAX_TB];
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int TB = pl.tb;
+  const uint32_t X_BYTES = (uint32_t)TB * 128u, stage_bytes = SUBTILE_BYTES + X_BYTES, T_BYTES = (uint32_t)TB * 32u, piece_bytes = LR_PIECE_BYTES + 2 * T_BYTES;
+  const uint32_t piece0 = sbase + (uint32_t)pl.stages * stage_bytes;
+  auto FULL = [&](int s) { return smem_u32(&bars[s]); };
+  auto EMPTY = [&](int s) { return smem_u32(&bars[LS_MAX_STAGES + s]); };
+  auto PFULL = [&](int s) { return smem_u32(&bars[2 * LS_MAX_STAGES + s]); };
+  auto PEMPTY = [&](int s) { return smem_u32(&bars[2 * LS_MAX_STAGES + LS_MAX_PIECES + s]); };
+  const uint32_t ACC = smem_u32(&bars[2 * LS_MAX_STAGES + 2 * LS_MAX_PIECES]);
+  const Ctl ctl{&s_abort, p.status};
+  const uint32_t tmem_cols = TB <= 32 ? 32u : TB <= 64 ? 64u : TB <= 128 ? 128u : 256u;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LS_MAX_STAGES; ++s) { mbar_init(FULL(s), 1); mbar_init(EMPTY(s), 1); }
+    for (int s = 0; s < LS_MAX_PIECES; ++s) { mbar_init(PFULL(s), 2); mbar_init(PEMPTY(s), 1); }
+    mbar_init(ACC, 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&w_map) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, s_tmem, 0);
+  pdl_begin();
+
+  const int n0 = blockIdx.x * LR_TILE_N, rank = blockIdx.z, S = pl.splits;
+  const int64_t row0 = (int64_t)blockIdx.y * TB;
+  const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0);
+  adapters_of(p, row0, rows, TB, s_idx, s_list, &s_count);
+  const int n_list = s_count;
+  for (int i = threadIdx.x; i < n_list; i += LS_THREADS) {
+    s_first[i] = p.first[s_list[i]];
+    s_np[i] = p.first[s_list[i] + 1] - s_first[i];
+  }
+  __syncthreads();
+  const int KT = (p.K + BLOCK_K - 1) / BLOCK_K, kt0 = KT * rank / S, kt1 = KT * (rank + 1) / S;
+  // the pieces of this CTA, every S-th of the block's: calls f(number, place in the list, piece of that adapter)
+  auto pieces = [&](auto f) {
+    int g = 0, mine = 0;
+    for (int l = 0; l < n_list; ++l)
+      for (int i = 0; i < s_np[l]; ++i, ++g)
+        if (g % S == rank && !f(mine++, l, i)) return;
+  };
+
+  if (warp == 0) {
+    // ================================= producer ================================================================
+    int it = 0, issued = 0;
+    bool ok = true;
+    auto piece = [&](int m, int l, int i) {
+      const int s = m % pl.pieces;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1101));
+      if (!ok) return false;
+      elect_expect_tx(PFULL(s), LR_PIECE_BYTES);
+      if (lane == 0) bulk_g2s(piece0 + (uint32_t)s * piece_bytes, p.b + ((int64_t)(s_first[l] + i) * p.NP + n0) * 32, LR_PIECE_BYTES, PFULL(s));
+      ++issued;
+      return true;
+    };
+    pieces([&](int m, int l, int i) { return m < pl.pieces && piece(m, l, i); });      // as many as the ring holds, ahead of the product
+    const int ahead = issued;
+    for (int kt = kt0; kt < kt1 && ok; ++kt, ++it) {
+      const int s = it % pl.stages;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(s), ((it / pl.stages) & 1u) ^ 1u, ctl, 1102));
+      if (!ok) break;
+      const uint32_t st = sbase + (uint32_t)s * stage_bytes;
+      elect_expect_tx(FULL(s), stage_bytes);
+      elect_tile_2d(st, &w_map, kt * BLOCK_K, n0, FULL(s));
+      elect_tile_2d(st + SUBTILE_BYTES, &x_map, kt * BLOCK_K, (int)row0, FULL(s));
+    }
+    if (ok) pieces([&](int m, int l, int i) { return m < ahead || piece(m, l, i); });
+    if (!ok && lane == 0) {                                   // copies in flight land before the block's shared memory goes
+      for (int j = it > pl.stages ? it - pl.stages : 0; j < it; ++j)
+        for (uint32_t w = 0; w < (1u << 16) && !mbar_test(FULL(j % pl.stages), (j / pl.stages) & 1u); ++w) __nanosleep(64);
+      __nanosleep(100000);                                    // (a piece's barrier also waits for its writer)
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ================================= MMA =====================================================================
+    int it = 0;
+    bool ok = true;
+    const uint32_t idesc = lr_idesc(std::is_same<T16, __half>::value, 128, TB);
+    for (int kt = kt0; kt < kt1; ++kt, ++it) {
+      const int s = it % pl.stages;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(FULL(s), (it / pl.stages) & 1u, ctl, 1103));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t st = sbase + (uint32_t)s * stage_bytes;
+      const uint32_t a_lo = DESC_LO | ((st & 0x3FFFFu) >> 4), b_lo = DESC_LO | (((st + SUBTILE_BYTES) & 0x3FFFFu) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) elect_mma_bf16(tmem, a_lo + kk * 2, b_lo + kk * 2, idesc, (it | kk) ? 1u : 0u);
+      elect_commit(EMPTY(s));
+    }
+    if (ok)
+      pieces([&](int m, int, int) {
+        const int s = m % pl.pieces;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(PFULL(s), (m / pl.pieces) & 1u, ctl, 1104));
+        if (!ok) return false;
+        tc_fence_after();
+        const uint32_t st = piece0 + (uint32_t)s * piece_bytes;
+        const uint32_t a_lo = piece_desc(st), b_lo = piece_desc(st + LR_PIECE_BYTES);
+        elect_mma_piece(tmem, a_lo, b_lo, idesc, (it | m) ? 1u : 0u);
+        elect_mma_piece(tmem, a_lo, b_lo + (T_BYTES >> 4), idesc, 1u);
+        elect_commit(PEMPTY(s));
+        return true;
+      });
+    elect_commit(ACC);
+    if (!ok)
+      for (uint32_t w = 0; w < (1u << 16) && !mbar_test(ACC, 0); ++w) __nanosleep(64);
+    __syncwarp();
+  } else if (warp < 6) {
+    // ================================= accumulator to shared memory: [token][output], over the ring ==================
+    if (__all_sync(0xFFFFFFFFu, mbar_wait(ACC, 0, ctl, 1105))) {
+      tc_fence_after();
+      const int qd = warp & 3;
+      float* part = reinterpret_cast<float*>(smem);
+      for (int c0 = 0; c0 < TB; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld16(tmem + (uint32_t)c0 + ((uint32_t)(qd * 32) << 16), v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * LR_TILE_N + qd * 32 + lane] = __uint_as_float(v[j]);
+      }
+    }
+    tc_fence_before();
+  } else {
+    // ================================= tokens' side of the pieces ===================================================
+    pieces([&](int m, int l, int i) {
+      const int s = m % pl.pieces;
+      if (s != warp - 6) return true;                         // a warp has a place of the ring: it sees every phase of its barrier
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1106))) return false;
+      const uint32_t dst = piece0 + (uint32_t)s * piece_bytes + LR_PIECE_BYTES;
+      for (int r = lane; r < TB; r += 32) write_piece_row<T16>(p, s_idx[r] == s_list[l], row0 + r, i * LR_PIECE, dst, T_BYTES, r);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(PFULL(s));
+      return true;
+    });
+  }
+  __syncthreads();
+  auto cluster_barrier = []() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
+  if (S > 1) cluster_barrier();
+  // ---- the cluster's shares of k meet, in their order: each CTA takes a share of the tokens ----
+  bool ok = true;
+  auto remote = [&](uint32_t at, int r) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(at), "r"(r) : "memory");
+    return v;
+  };
+  for (int r = 0; r < S; ++r) ok = ok && (S > 1 ? remote(smem_u32(&s_abort), r) : (uint32_t)s_abort) == 0;
+  if (ok) {
+    const int t0 = rows * rank / S, t1 = rows * (rank + 1) / S;
+    for (int i = threadIdx.x; i < (t1 - t0) * LR_TILE_N; i += LS_THREADS) {
+      const int tok = t0 + (i >> 7), n = n0 + (i & 127);
+      if (n >= p.N) continue;
+      const uint32_t at = sbase + (uint32_t)(tok * LR_TILE_N + (i & 127)) * 4u;
+      float v = 0.0f;
+      for (int r = 0; r < S; ++r) v += __uint_as_float(S > 1 ? remote(at, r) : lds32(at));
+      if (p.bias) v += load_bias(p.bias, p.bias_dtype, n);
+      ((T16*)p.y)[(row0 + tok) * p.ld_y + n] = from_f32<T16>(v);
+    }
+  }
+  if (S > 1) cluster_barrier();                               // no CTA leaves while its sums are read
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------
+// rows of K 16-bit values as boxes of 64 x box_rows in the 128-byte swizzle; zeros outside
+int lr_map(const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows, bool f16, CUtensorMap* map) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!encode) {
+      void* fn = nullptr;
+      cudaDriverEntryPointQueryResult qr;
+      MOE_CHECK_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &qr));
+      if (qr != cudaDriverEntryPointSuccess || !fn) {
+        moe_set_error("moe_lora_matmul: the driver does not provide cuTensorMapEncodeTiled");
+        return MOE_ERR_UNSUPPORTED;
+      }
+      encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+    }
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    moe_set_error("moe_lora_matmul: cuTensorMapEncodeTiled failed with code %d (rows %lld, K %lld, pitch %lld)", (int)r, (long long)rows, (long long)K, (long long)ld);
+    return MOE_ERR_CUDA;
+  }
+  return MOE_OK;
+}
+
+struct ShrinkPlan { int nb, places, parts; };
+ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
+  ShrinkPlan s;
+  s.nb = T <= 128 ? 1 : 8;
+  const int64_t blocks = cdiv64(T, 8 * s.nb);
+  const int64_t most = n_adapters < 8 * s.nb ? n_adapters : 8 * s.nb;             // adapters that a block can hold
+  s.places = (int)(most < (s.nb == 1 ? 8 : 4) ? most : (s.nb == 1 ? 8 : 4));
+  if (s.places < 1) s.places = 1;
+  // shares of k while there are fewer CTAs than SMs
+  int parts = 1;
+  while (parts < 8 && blocks * max_pieces * s.places * parts * 2 <= moe_sm_count() && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
+  s.parts = parts;
+  return s;
+}
+
+StreamPlan lr_stream_plan(int64_t T, int K, int N) {
+  StreamPlan pl;
+  pl.tb = T >= LS_MAX_TB ? LS_MAX_TB : (int)cdiv64(T, 16) * 16;
+  const int64_t tiles = cdiv64(N, LR_TILE_N) * cdiv64(T, pl.tb), KT = cdiv64(K, BLOCK_K);
+  const int stage = SUBTILE_BYTES + pl.tb * 128, piece = LR_PIECE_BYTES + pl.tb * 64;
+  // two CTAs per SM while the accumulator and a ring of four steps leave room for them: they fill the SMs more evenly
+  const bool two = pl.tb <= 64;
+  const int room = (two ? 112 : 224) * 1024 - 8 * 1024;
+  int64_t s = (two ? 2 : 1) * moe_sm_count() / tiles;
+  if (s > KT / 4) s = KT / 4;
+  pl.splits = (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+  pl.pieces = pl.tb <= 64 ? 4 : 2;
+  int st = (room - pl.pieces * piece) / stage;
+  pl.stages = st > LS_MAX_STAGES ? LS_MAX_STAGES : st;
+  int bytes = pl.stages * stage + pl.pieces * piece;
+  if (bytes < pl.tb * LR_TILE_N * 4) bytes = pl.tb * LR_TILE_N * 4;
+  pl.smem = bytes + 1024;
+  return pl;
+}
+
+size_t lr_t_bytes(const MoeLoraArgs& a, ShrinkPlan s) { return (size_t)s.parts * (size_t)a.T * (size_t)a.max_pieces * LR_PIECE * 4; }
+
+int lr_check(const MoeLoraArgs* a) {
+  MOE_CHECK_ARG(a, "moe_lora_matmul: NULL argument");
+  MOE_CHECK_ARG(a->T >= 0 && a->K > 0 && a->N > 0 && a->n_adapters >= 0 && a->max_pieces >= 0, "moe_lora_matmul: sizes must be positive");
+  MOE_CHECK_ARG(a->dtype == MOE_BF16 || a->dtype == MOE_F16, "moe_lora_matmul: x, W and the adapters are bf16 or fp16");
+  if (a->T >= (1ll << 31) - 512 || a->K > (1 << 30) || a->N > (1 << 30) || a->max_pieces > 64) {
+    moe_set_error("moe_lora_matmul: takes fewer than 2^31 tokens and ranks up to 1024 (got T = %lld, K = %d, N = %d, %d pieces of 16 ranks)", (long long)a->T, a->K,
+                  a->N, a->max_pieces);
+    return MOE_ERR_UNSUPPORTED;
+  }
+  return MOE_OK;
+}
+
+template <typename T16> int lr_shrink(const LoraParams& p, const ShrinkPlan& sp, cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv64(p.T, 8 * sp.nb), (unsigned)p.max_pieces, (unsigned)(sp.places * sp.parts));
+  if (sp.nb == 1) MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 1>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
+  else MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 8>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+template <typename T16> int lr_stream(const LoraParams& p, const MoeLoraArgs& a, cudaStream_t st) {
+  const bool f16 = std::is_same<T16, __half>::value;
+  const StreamPlan pl = lr_stream_plan(p.T, p.K, p.N);
+  CUtensorMap w_map, x_map;
+  if (int rc = lr_map(a.w_t, a.N, a.K, a.ld_w, LR_TILE_N, f16, &w_map)) return rc;
+  if (int rc = lr_map(a.x, a.T, a.K, a.ld_x, pl.tb, f16, &x_map)) return rc;
+  MOE_CHECK_CUDA(cudaFuncSetAttribute(lora_stream_kernel<T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cdiv64(p.N, LR_TILE_N), (unsigned)cdiv64(p.T, pl.tb), (unsigned)pl.splits);
+  cfg.blockDim = dim3(LS_THREADS);
+  cfg.dynamicSmemBytes = (size_t)pl.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 1; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = (unsigned)pl.splits;
+  cfg.attrs = at;
+  cfg.numAttrs = pl.splits > 1 ? 2 : 1;
+  MOE_CHECK_CUDA(cudaLaunchKernelEx(&cfg, lora_stream_kernel<T16>, p, pl, w_map, x_map));
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) size_t moe_lora_matmul_workspace_bytes(const MoeLoraArgs* a) {
+  if (lr_check(a) != MOE_OK || a->n_adapters == 0) return 0;
+  return lr_t_bytes(*a, lr_shrink_plan(a->T, a->K, a->max_pieces, a->n_adapters));
+}
+
+extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeLoraArgs* args, void* stream) {
+  if (int rc = lr_check(args)) return rc;
+  const MoeLoraArgs& a = *args;
+  if (a.T == 0) return MOE_OK;
+  MOE_CHECK_ARG(a.x && a.w_t && a.y, "moe_lora_matmul: NULL argument");
+  MOE_CHECK_ARG(a.ld_x % 8 == 0 && a.ld_w % 8 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w_t % 16 == 0,
+                "moe_lora_matmul: rows of x and W^T must be 16-byte aligned");
+  const bool adapters = a.n_adapters > 0 && a.max_pieces > 0;
+  ShrinkPlan sp = {1, 1, 1};
+  if (adapters) {
+    MOE_CHECK_ARG(a.a && a.b && a.first && a.scale && a.indx, "moe_lora_matmul: NULL argument of the adapters");
+    MOE_CHECK_ARG(a.ld_a % 8 == 0 && a.ld_a >= (a.K + 7) / 8 * 8 && (uintptr_t)a.a % 16 == 0 && (uintptr_t)a.b % 16 == 0,
+                  "moe_lora_matmul: adapters must be 16-byte aligned, their rows padded to 8 values");
+    MOE_CHECK_ARG(a.ld_x >= (a.K + 7) / 8 * 8, "moe_lora_matmul: rows of x must be padded to 8 values");
+    sp = lr_shrink_plan(a.T, a.K, a.max_pieces, a.n_adapters);
+    MOE_CHECK_ARG(a.workspace && (uintptr_t)a.workspace % 256 == 0 && a.workspace_bytes >= lr_t_bytes(a, sp),
+                  "moe_lora_matmul: needs a 256-byte aligned workspace of %zu bytes", lr_t_bytes(a, sp));
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  LoraParams p = {};
+  p.x = a.x; p.ld_x = a.ld_x; p.T = (int)a.T; p.K = a.K; p.N = a.N; p.NP = (int)cdiv64(a.N, LR_TILE_N) * LR_TILE_N;
+  p.bias = a.bias; p.bias_dtype = a.bias_dtype;
+  if (adapters) {
+    p.a = a.a; p.ld_a = a.ld_a; p.b = (const uint8_t*)a.b; p.first = a.first; p.scale = a.scale; p.n_adapters = a.n_adapters; p.max_pieces = a.max_pieces;
+    p.indx = a.indx;
+    p.t = (float*)a.workspace; p.ld_t = (int64_t)a.max_pieces * LR_PIECE; p.t_parts = sp.parts; p.t_part_stride = a.T * p.ld_t;
+  }
+  p.y = a.y; p.ld_y = a.ld_y; p.status = a.status;
+  if (adapters)
+    if (int rc = a.dtype == MOE_F16 ? lr_shrink<__half>(p, sp, st) : lr_shrink<__nv_bfloat16>(p, sp, st)) return rc;
+  return a.dtype == MOE_F16 ? lr_stream<__half>(p, a, st) : lr_stream<__nv_bfloat16>(p, a, st);
+}

@@ -130,6 +130,9 @@ _STATUS_TEXT = {
     1001: "layer of a few tokens: the weight producer waited for a free stage", 1002: "layer of a few tokens: a warp waited for weights",
     1003: "layer of a few tokens: fc2 waited for fc1's rows", 1004: "layer of a few tokens: the combine waited for fc2's sums",
     1005: "layer of a few tokens: the epilogue waited for a unit's sums", 1006: "layer of a few tokens: a warp waited for a free buffer of sums",
+    1101: "projection with adapters: the producer waited for a free piece", 1102: "projection with adapters: the producer waited for a free stage",
+    1103: "projection with adapters: the MMA warp waited for a stage", 1104: "projection with adapters: the MMA warp waited for a piece",
+    1105: "projection with adapters: the epilogue waited for the accumulator", 1106: "projection with adapters: a writer waited for a free piece",
 }
 
 
@@ -140,7 +143,7 @@ def status_message(code: int) -> str:
 
 def matmul_check_status(device=None):
     """Synchronise and raise if a bounded wait expired since the last check: a pipeline wait inside a tensor-core
-    kernel (codes 1xx-8xx and 10xx) or an expert-parallel peer barrier (901).  Expert-parallel callers should poll this once
+    kernel (codes 1xx-8xx, 10xx and 11xx) or an expert-parallel peer barrier (901).  Expert-parallel callers should poll this once
     per step or batch: after a barrier time-out the step carries on with stale peer buffers and its result is wrong."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     w = _status_word(dev)
