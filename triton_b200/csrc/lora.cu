@@ -11,7 +11,7 @@
 //     terms (hi + lo, 16 bits of it in bf16), so it costs the result nothing.
 // The second has two forms: lora_stream_kernel for few tokens (weight rows are the MMA's 128 rows, up to 256 tokens its columns, K cut over a cluster) and
 // lora_pair_kernel for many (a pair of SMs per tile of 256 tokens x 256 outputs).
-#include "gemm_tc_common.cuh"
+#include "gemm_pair_common.cuh"
 #include <cuda_fp16.h>
 #include <type_traits>
 
@@ -30,8 +30,10 @@ struct LoraParams {
   const int32_t* indx;
   float* t; int64_t ld_t; int t_parts; int64_t t_part_stride;     // shares of k whose sums make up t
   void* y; int64_t ld_y;
+  int32_t* list; int list_tb;                          // the adapters of every block of list_tb tokens: [LR_LIST] their count, then they
   int32_t* status;
 };
+constexpr int LR_MAX_TB = 512, LR_LIST = LR_MAX_TB + 4;
 
 // ---- shrink ----------------------------------------------------------------------------------------------------
 template <typename T16> __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -50,22 +52,23 @@ __device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, i
     const int a = r < rows && p.indx ? p.indx[row0 + r] : -1;
     idx[r] = a >= 0 && a < p.n_adapters ? a : -1;
   }
-  if (threadIdx.x == 0) *count = 0;
   __syncthreads();
-  for (int r0 = 0; r0 < block_rows; r0 += 32) {             // one warp, 32 tokens at a time
-    if (threadIdx.x >= 32) break;
-    const int r = r0 + threadIdx.x, a = r < block_rows ? idx[r] : -1;
-    bool fresh = a >= 0;
-    const int n = *count;
-    for (int i = 0; i < n && fresh; ++i) fresh = list[i] != a;
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, a);
-    fresh = fresh && (int)threadIdx.x == __ffs(same) - 1;
-    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, fresh);
-    __syncwarp();
-    if (fresh) list[n + __popc(mask & ((1u << threadIdx.x) - 1u))] = a;
-    __syncwarp();
-    if (threadIdx.x == 0) *count = n + __popc(mask);
-    __syncwarp();
+  for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {          // an adapter counts at its first token
+    bool fresh = idx[r] >= 0;
+    for (int i = 0; i < r && fresh; ++i) fresh = idx[i] != idx[r];
+    list[r] = fresh ? idx[r] : -1;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int n = 0;
+    for (int r0 = 0; r0 < block_rows; r0 += 32) {
+      const int r = r0 + threadIdx.x, a = r < block_rows ? list[r] : -1;
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, a >= 0);
+      if (a >= 0) list[n + __popc(mask & ((1u << threadIdx.x) - 1u))] = a;      // (at or before where it was read)
+      n += __popc(mask);
+      __syncwarp();
+    }
+    if (threadIdx.x == 0) *count = n;
   }
   __syncthreads();
 }
@@ -76,7 +79,7 @@ constexpr int SH_WARPS = 8;
 template <typename T16, int NB>
 __global__ void __launch_bounds__(SH_WARPS * 32) lora_shrink_kernel(const LoraParams p, const int places) {
   __shared__ int s_idx[8 * NB], s_list[8 * NB], s_count;
-  __shared__ float s_sum[SH_WARPS][NB][32][4];
+  __shared__ __align__(16) float s_sum[SH_WARPS][NB][32][4];
   pdl_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qrow = lane >> 2, c4 = lane & 3;
   const int64_t row0 = (int64_t)blockIdx.x * (8 * NB);
@@ -135,7 +138,18 @@ __global__ void __launch_bounds__(SH_WARPS * 32) lora_shrink_kernel(const LoraPa
     }
     __syncthreads();
   }
+  // the adapters of the product's blocks of tokens, for its kernel
+  if (p.list_tb > 0 && blockIdx.y == 0 && blockIdx.z == 0 && (int64_t)blockIdx.x * p.list_tb < p.T) {
+    int* idx = reinterpret_cast<int*>(s_sum);
+    const int64_t first = (int64_t)blockIdx.x * p.list_tb;
+    __syncthreads();
+    adapters_of(p, first, (int)min((int64_t)p.list_tb, (int64_t)p.T - first), p.list_tb, idx, idx + LR_MAX_TB, &s_count);
+    int32_t* out = p.list + (int64_t)blockIdx.x * LR_LIST;
+    for (int i = threadIdx.x; i < s_count; i += SH_WARPS * 32) out[1 + i] = idx[LR_MAX_TB + i];
+    if (threadIdx.x == 0) out[0] = s_count;
+  }
 }
+static_assert(2 * LR_MAX_TB * sizeof(int) <= SH_WARPS * 32 * 4 * sizeof(float), "lists in place of the sums");
 
 // ---- pieces as MMA operands --------------------------------------------------------------------------------------
 // Operands of 16 k without swizzle: eight rows of 16 bytes are 128 bytes in a row, the two halves of k follow one another, then the next eight rows.
@@ -198,7 +212,7 @@ __device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, 
 
 // ---- few tokens ------------------------------------------------------------------------------------------------
 constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-5 epilogue, 6-9 write the tokens' side of the pieces
-constexpr int LS_MAX_STAGES = 8, LS_MAX_PIECES = 4, LS_MAX_TB = 256;
+constexpr int LS_MAX_STAGES = 8, LS_MAX_PIECES = 4, LS_MAX_TB = 64;
 
 struct StreamPlan { int tb, splits, stages, pieces, smem; };      // tokens of a block, cluster, ring of k steps, ring of pieces, bytes
 
@@ -387,6 +401,264 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
   }
 }
 
+// ---- many tokens -----------------------------------------------------------------------------------------------
+// A cluster of two CTAs computes 256 outputs x up to 512 tokens with tcgen05.mma.cta_group::2: weight rows are the MMA's 256 rows (128 in each CTA),
+// tokens its columns, in one or two MMAs of up to 256.  What bounds it is the way from L2 into an SM, some 43 B/ns (no operand is shared between
+// clusters): a k step of 64 brings (128 + tb / 2) rows of 128 bytes into each SM, so the tile is as large as tensor memory, one accumulator
+// at a time, and the ring is filled again while it is drained.  With few tiles k is cut over up to four pairs of a larger cluster, whose sums meet through distributed
+// shared memory as in the kernel above.
+constexpr int LP_THREADS = 320, LP_MAX_STAGES = 4, LP_MAX_PIECES = 4;
+struct PairPlan { int tb, mmas, splits, stages, pieces, tiles_n, blocks, clusters, smem; };
+
+__device__ __forceinline__ void elect_mma_pair_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(hi)
+      : "memory");
+}
+// arrive on the barrier at this offset in both CTAs of this pair once every MMA issued so far has completed
+__device__ __forceinline__ void elect_commit_both(uint32_t bar, uint32_t mask) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+      "h"((uint16_t)mask)
+      : "memory");
+}
+// a tile into this CTA's shared memory whose bytes count on the barrier of the pair's even CTA
+__device__ __forceinline__ void elect_tile_pair(uint32_t dst, const CUtensorMap* tmap, int col, int row, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+      "l"(tmap), "r"(col), "r"(row), "r"(bar & 0xFEFFFFFFu)
+      : "memory");
+}
+
+template <typename T16>
+__global__ void __launch_bounds__(LP_THREADS, 1)
+lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem);
+  __shared__ __align__(8) uint64_t bars[2 * LP_MAX_STAGES + 3 * LP_MAX_PIECES + 3];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank(), half_id = crank & 1u, even = crank & ~1u, both = 3u << even;
+  const int S = pl.splits, split = (int)(crank >> 1), TB = pl.tb, n_mma = TB / pl.mmas, half = n_mma / 2;
+  const uint32_t X_BYTES = (uint32_t)(TB / 2) * 128u, stage_bytes = SUBTILE_BYTES + X_BYTES, T_BYTES = (uint32_t)(TB / 2) * 32u,
+                 piece_bytes = LR_PIECE_BYTES + 2 * T_BYTES;
+  const uint32_t piece0 = sbase + (uint32_t)pl.stages * stage_bytes;
+  auto FULL = [&](int s) { return smem_u32(&bars[s]); };                                   // of the even CTA: both CTAs' tiles
+  auto EMPTY = [&](int s) { return smem_u32(&bars[LP_MAX_STAGES + s]); };
+  auto PTILE = [&](int s) { return smem_u32(&bars[2 * LP_MAX_STAGES + s]); };              // B's tile of a piece in this CTA
+  auto PFULL = [&](int s) { return smem_u32(&bars[2 * LP_MAX_STAGES + LP_MAX_PIECES + s]); };      // of the even CTA: the piece in both
+  auto PEMPTY = [&](int s) { return smem_u32(&bars[2 * LP_MAX_STAGES + 2 * LP_MAX_PIECES + s]); };
+  const uint32_t ACC = smem_u32(&bars[2 * LP_MAX_STAGES + 3 * LP_MAX_PIECES]), ACC_FREE = ACC + 8u, DRAIN = ACC + 16u;
+  const Ctl ctl{&s_abort, p.status};
+  const uint32_t tmem_cols = TB <= 64 ? 64u : TB <= 128 ? 128u : TB <= 256 ? 256u : 512u;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LP_MAX_STAGES; ++s) { mbar_init(FULL(s), 1); mbar_init(EMPTY(s), 1); }
+    for (int s = 0; s < LP_MAX_PIECES; ++s) { mbar_init(PTILE(s), 1); mbar_init(PFULL(s), 8); mbar_init(PEMPTY(s), 1); }
+    mbar_init(ACC, 1);
+    mbar_init(ACC_FREE, 8);
+    mbar_init(DRAIN, 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&w_map) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                         // every CTA's barriers exist before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, s_tmem, 0);
+  pdl_begin();
+
+  const int KT = (p.K + BLOCK_K - 1) / BLOCK_K, kt0 = KT * split / S, kt1 = KT * (split + 1) / S;
+  const int tiles = pl.tiles_n * pl.blocks, me = blockIdx.x / (2 * S);
+  // consecutive tiles have the same tokens; one tile per cluster where k is cut
+  const int tile0 = (int)((int64_t)tiles * me / pl.clusters), tile1 = (int)((int64_t)tiles * (me + 1) / pl.clusters);
+  // this split's pieces of a token block: calls f(number, adapter, piece of that adapter); `m` runs on over the tiles
+  auto pieces = [&](int block, int& m, auto f) {
+    if (p.list == nullptr) return true;
+    const int32_t* list = p.list + (int64_t)block * LR_LIST;
+    const int n = list[0];
+    int g = 0;
+    for (int l = 0; l < n; ++l) {
+      const int a = list[1 + l], np = p.first[a + 1] - p.first[a];
+      for (int i = 0; i < np; ++i, ++g)
+        if (g % S == split) {
+          if (!f(m, a, i)) return false;
+          ++m;
+        }
+    }
+    return true;
+  };
+
+  if (warp == 0) {
+    // ================================= producer ================================================================
+    int it = 0, m = 0;
+    bool ok = true;
+    for (int tile = tile0; tile < tile1 && ok; ++tile) {
+      const int block = tile / pl.tiles_n, n0 = (tile - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
+      for (int kt = kt0; kt < kt1; ++kt, ++it) {
+        const int s = it % pl.stages;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(s), ((it / pl.stages) & 1u) ^ 1u, ctl, 1111));
+        if (!ok) break;
+        const uint32_t st = sbase + (uint32_t)s * stage_bytes;
+        if (half_id == 0) elect_expect_tx(FULL(s), 2 * stage_bytes);
+        elect_tile_pair(st, &w_map, kt * BLOCK_K, n0, FULL(s));
+        for (int j = 0; j < pl.mmas; ++j)
+          elect_tile_pair(st + SUBTILE_BYTES + (uint32_t)(j * half) * 128u, &x_map, kt * BLOCK_K, block * TB + j * n_mma + (int)half_id * half, FULL(s));
+      }
+      ok = ok && pieces(block, m, [&](int m, int a, int i) {
+        const int s = m % pl.pieces;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1112))) return false;
+        elect_expect_tx(PTILE(s), LR_PIECE_BYTES);
+        // (rows of B are padded to 128: the odd CTA of the last tile may have none)
+        const int64_t at = ((int64_t)(p.first[a] + i) * p.NP + (n0 < p.NP ? n0 : 0)) * 32;
+        if (lane == 0) bulk_g2s(piece0 + (uint32_t)s * piece_bytes, p.b + at, LR_PIECE_BYTES, PTILE(s));
+        return true;
+      });
+    }
+    if (!ok) __nanosleep(500000);                             // copies in flight land before the block's shared memory goes
+    __syncwarp();
+  } else if (warp == 1) {
+    if (half_id == 0) {
+      // ================================= MMA ===================================================================
+      int it = 0, m = 0;
+      bool ok = true;
+      const uint32_t idesc = lr_idesc(std::is_same<T16, __half>::value, 256, n_mma);
+      for (int tile = tile0, tc = 0; tile < tile1 && ok; ++tile, ++tc) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(ACC_FREE, (tc & 1u) ^ 1u, ctl, 1113));
+        if (!ok) break;
+        tc_fence_after();
+        for (int kt = kt0; kt < kt1; ++kt, ++it) {
+          const int s = it % pl.stages;
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(FULL(s), (it / pl.stages) & 1u, ctl, 1114));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = (sbase + (uint32_t)s * stage_bytes) & 0x3FFFFu, a_lo = DESC_LO | (st >> 4), b_lo = DESC_LO | ((st + SUBTILE_BYTES) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            for (int j = 0; j < pl.mmas; ++j)
+              elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo + kk * 2, b_lo + (uint32_t)(j * half * 8) + kk * 2, DESC_HI, idesc, kt > kt0 || kk > 0 ? 1u : 0u);
+          elect_commit_both(EMPTY(s), both);
+        }
+        ok = ok && pieces(tile / pl.tiles_n, m, [&](int m, int, int) {
+          const int s = m % pl.pieces;
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(PFULL(s), (m / pl.pieces) & 1u, ctl, 1115))) return false;
+          tc_fence_after();
+          const uint32_t st = piece0 + (uint32_t)s * piece_bytes, a_lo = piece_desc(st), b_lo = piece_desc(st + LR_PIECE_BYTES);
+          for (int j = 0; j < pl.mmas; ++j) {
+            elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo, b_lo + (uint32_t)(j * half * 2), PIECE_DESC_HI, idesc, 1u);
+            elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo, b_lo + (T_BYTES >> 4) + (uint32_t)(j * half * 2), PIECE_DESC_HI, idesc, 1u);
+          }
+          elect_commit_both(PEMPTY(s), both);
+          return true;
+        });
+        if (ok) elect_commit_both(ACC, both);
+      }
+      elect_commit_pair_local(DRAIN);                         // every MMA has retired before tensor memory is freed
+      for (uint32_t w = 0; w < (1u << 16) && !mbar_test(DRAIN, 0); ++w) __nanosleep(64);
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    // ================================= epilogue ================================================================
+    const int qd = warp & 3;
+    for (int tile = tile0, tc = 0; tile < tile1; ++tile, ++tc) {
+      const int block = tile / pl.tiles_n, n = (tile - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N + qd * 32 + lane;
+      const int64_t row0 = (int64_t)block * TB;
+      const int cols = (int)min((int64_t)TB, (int64_t)p.T - row0);
+      const float bias = S == 1 && p.bias && n < p.N ? load_bias(p.bias, p.bias_dtype, n) : 0.0f;
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(ACC, tc & 1u, ctl, 1116))) break;
+      tc_fence_after();
+      float* part = reinterpret_cast<float*>(smem);
+      for (int c0 = 0; c0 < cols; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem + (uint32_t)c0 + ((uint32_t)(qd * 32) << 16), v);
+        tmem_ld_wait();
+        if (S > 1) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[(c0 + j) * LR_TILE_N + qd * 32 + lane] = __uint_as_float(v[j]);
+        } else if (n < p.N) {
+          T16* y = (T16*)p.y + (row0 + c0) * p.ld_y + n;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < cols) y[j * p.ld_y] = from_f32<T16>(__uint_as_float(v[j]) + bias);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(ACC_FREE, even);
+    }
+  } else {
+    // ================================= tokens' side of the pieces ===================================================
+    int m = 0;
+    bool ok = true;
+    for (int tile = tile0; tile < tile1 && ok; ++tile) {
+      const int block = tile / pl.tiles_n;
+      ok = pieces(block, m, [&](int m, int a, int i) {
+        const int s = m % pl.pieces;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1117))) return false;
+        const uint32_t dst = piece0 + (uint32_t)s * piece_bytes + LR_PIECE_BYTES;
+        for (int r = (warp - 6) * 32 + lane; r < TB / 2; r += 128) {
+          const int j = r >= half ? 1 : 0;
+          const int64_t token = (int64_t)block * TB + j * n_mma + (int)half_id * half + (r - j * half);
+          write_piece_row<T16>(p, token < p.T && p.indx[token] == a, token, i * LR_PIECE, dst, T_BYTES, r);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (warp == 6 && !__all_sync(0xFFFFFFFFu, mbar_wait(PTILE(s), (m / pl.pieces) & 1u, ctl, 1118))) return false;
+        if (lane == 0) mbar_arrive_cluster(PFULL(s), even);
+        return true;
+      });
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (S > 1) {
+    // ---- the splits' sums meet, in their order: each CTA takes a share of the tokens of its half of the outputs ----
+    auto remote = [&](uint32_t at, uint32_t r) {
+      uint32_t v;
+      asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(at), "r"(r) : "memory");
+      return v;
+    };
+    bool ok = true;
+    for (int r = 0; r < 2 * S; ++r) ok = ok && remote(smem_u32(&s_abort), (uint32_t)r) == 0;
+    if (ok && tile0 < tile1) {
+      const int block = tile0 / pl.tiles_n, n0 = (tile0 - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
+      const int64_t row0 = (int64_t)block * TB;
+      const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0), t0 = rows * split / S, t1 = rows * (split + 1) / S;
+      for (int i = threadIdx.x; i < (t1 - t0) * LR_TILE_N; i += LP_THREADS) {
+        const int tok = t0 + (i >> 7), n = n0 + (i & 127);
+        if (n >= p.N) continue;
+        const uint32_t at = sbase + (uint32_t)(tok * LR_TILE_N + (i & 127)) * 4u;
+        float v = 0.0f;
+        for (int r = 0; r < S; ++r) v += __uint_as_float(remote(at, (uint32_t)(2 * r) + half_id));
+        if (p.bias) v += load_bias(p.bias, p.bias_dtype, n);
+        ((T16*)p.y)[(row0 + tok) * p.ld_y + n] = from_f32<T16>(v);
+      }
+    }
+    cluster_sync_all();                                       // no CTA leaves while its sums are read
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------
 // rows of K 16-bit values as boxes of 64 x box_rows in the 128-byte swizzle; zeros outside
 int lr_map(const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows, bool f16, CUtensorMap* map) {
@@ -439,14 +711,13 @@ StreamPlan lr_stream_plan(int64_t T, int K, int N) {
   pl.tb = T >= LS_MAX_TB ? LS_MAX_TB : (int)cdiv64(T, 16) * 16;
   const int64_t tiles = cdiv64(N, LR_TILE_N) * cdiv64(T, pl.tb), KT = cdiv64(K, BLOCK_K);
   const int stage = SUBTILE_BYTES + pl.tb * 128, piece = LR_PIECE_BYTES + pl.tb * 64;
-  // two CTAs per SM while the accumulator and a ring of four steps leave room for them: they fill the SMs more evenly
-  const bool two = pl.tb <= 64;
-  const int room = (two ? 112 : 224) * 1024 - 8 * 1024;
-  int64_t s = (two ? 2 : 1) * moe_sm_count() / tiles;
+  // Two CTAs per SM.  k is cut as long as the clusters fit side by side, which they do not up to the last place: 40 tiles took 21.5 us in clusters of four
+  // to six CTAs and 29.7 in clusters of seven (280 CTAs of 296), where some wait for a second round.
+  int64_t s = moe_sm_count() * 5 / 3 / tiles;
   if (s > KT / 4) s = KT / 4;
-  pl.splits = (int)(s < 1 ? 1 : s > 8 ? 8 : s);
-  pl.pieces = pl.tb <= 64 ? 4 : 2;
-  int st = (room - pl.pieces * piece) / stage;
+  pl.splits = (int)(s < 1 ? 1 : s > 6 ? 6 : s);
+  pl.pieces = LS_MAX_PIECES;
+  const int st = (104 * 1024 - pl.pieces * piece) / stage;
   pl.stages = st > LS_MAX_STAGES ? LS_MAX_STAGES : st;
   int bytes = pl.stages * stage + pl.pieces * piece;
   if (bytes < pl.tb * LR_TILE_N * 4) bytes = pl.tb * LR_TILE_N * 4;
@@ -454,7 +725,72 @@ StreamPlan lr_stream_plan(int64_t T, int K, int N) {
   return pl;
 }
 
-size_t lr_t_bytes(const MoeLoraArgs& a, ShrinkPlan s) { return (size_t)s.parts * (size_t)a.T * (size_t)a.max_pieces * LR_PIECE * 4; }
+// Clusters of 2 s CTAs of the pair kernel that run side by side (asked once per device)
+int64_t lr_pair_clusters(int s) {
+  static std::mutex mu;
+  static int cached[64][5] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  std::lock_guard<std::mutex> lk(mu);
+  if (cached[dev][s] == 0) {
+    const int smem = 225 * 1024;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * s * 256));
+    cfg.blockDim = dim3(LP_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)(2 * s); at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(lora_pair_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, lora_pair_kernel<__nv_bfloat16>, &cfg) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = moe_sm_count() / (2 * s) > 0 ? moe_sm_count() / (2 * s) : 1;
+    }
+    cached[dev][s] = n;
+  }
+  return cached[dev][s];
+}
+
+// Form of the product for many tokens.  Tokens are cut into blocks and k over up to four pairs; a round of tiles costs what comes into an SM, in rows of
+// 128 bytes, and draining the accumulator about as much as 2.6 rows a token.
+PairPlan lr_pair_plan(int64_t T, int K, int N) {
+  PairPlan best = {};
+  const int64_t pairs = lr_pair_clusters(1), KT = cdiv64(K, BLOCK_K), tiles_n = cdiv64(N, 256);
+  double least = 0.0;
+  const int64_t fewest = cdiv64(T, LR_MAX_TB);
+  for (int64_t nb = fewest; nb <= 2 * fewest + 6; ++nb) {
+    int64_t tb = cdiv64(cdiv64(T, nb), 32) * 32;
+    if (tb < 64) tb = 64;
+    const int64_t blocks = cdiv64(T, tb), tiles = tiles_n * blocks;
+    int64_t s = tb > 416 ? 1 : KT / 4 < 4 ? KT / 4 : 4;       // (a split's sums are tb x 128 fp32 in shared memory)
+    while (s > 1 && tiles > lr_pair_clusters((int)s)) --s;
+    if (s < 1) s = 1;
+    const double rounds = (double)cdiv64(tiles, lr_pair_clusters((int)s));
+    const double cost = rounds * ((double)cdiv64(KT, s) * (128 + tb / 2) + 2.6 * tb);
+    if (best.tb == 0 || cost < least) {
+      least = cost;
+      best.tb = (int)tb; best.blocks = (int)blocks; best.splits = (int)s; best.tiles_n = (int)tiles_n;
+      best.clusters = (int)(s > 1 || tiles < pairs ? tiles : pairs);
+    }
+  }
+  best.mmas = best.tb > 256 ? 2 : 1;
+  const int stage = SUBTILE_BYTES + best.tb * 64, piece = LR_PIECE_BYTES + best.tb * 32, room = 224 * 1024;
+  best.pieces = best.tb > 256 ? 2 : 4;
+  best.stages = (room - best.pieces * piece) / stage;
+  if (best.stages > LP_MAX_STAGES) best.stages = LP_MAX_STAGES;
+  int bytes = best.stages * stage + best.pieces * piece;
+  if (best.splits > 1 && bytes < best.tb * LR_TILE_N * 4) bytes = best.tb * LR_TILE_N * 4;
+  best.smem = bytes + 1024;
+  return best;
+}
+// Up to 64 tokens weight rows by themselves fill the SMs (two CTAs each); beyond, a pair reads the tokens half as often.
+bool lr_many(int64_t T) { return T > 64; }
+
+size_t lr_t_bytes(const MoeLoraArgs& a, ShrinkPlan s) { return ((size_t)s.parts * (size_t)a.T * (size_t)a.max_pieces * LR_PIECE * 4 + 255) / 256 * 256; }
+size_t lr_list_bytes(const MoeLoraArgs& a) { return lr_many(a.T) ? (size_t)lr_pair_plan(a.T, a.K, a.N).blocks * LR_LIST * 4 : 0; }
 
 int lr_check(const MoeLoraArgs* a) {
   MOE_CHECK_ARG(a, "moe_lora_matmul: NULL argument");
@@ -500,11 +836,34 @@ template <typename T16> int lr_stream(const LoraParams& p, const MoeLoraArgs& a,
   return MOE_OK;
 }
 
+template <typename T16> int lr_pair(const LoraParams& p, const MoeLoraArgs& a, const PairPlan& pl, cudaStream_t st) {
+  const bool f16 = std::is_same<T16, __half>::value;
+  CUtensorMap w_map, x_map;
+  if (int rc = lr_map(a.w_t, a.N, a.K, a.ld_w, LR_TILE_N, f16, &w_map)) return rc;
+  if (int rc = lr_map(a.x, a.T, a.K, a.ld_x, pl.tb / pl.mmas / 2, f16, &x_map)) return rc;
+  MOE_CHECK_CUDA(cudaFuncSetAttribute(lora_pair_kernel<T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pl.clusters * 2 * pl.splits));
+  cfg.blockDim = dim3(LP_THREADS);
+  cfg.dynamicSmemBytes = (size_t)pl.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)(2 * pl.splits); at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  MOE_CHECK_CUDA(cudaLaunchKernelEx(&cfg, lora_pair_kernel<T16>, p, pl, w_map, x_map));
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
 }  // namespace
 
 extern "C" __attribute__((visibility("default"))) size_t moe_lora_matmul_workspace_bytes(const MoeLoraArgs* a) {
   if (lr_check(a) != MOE_OK || a->n_adapters == 0) return 0;
-  return lr_t_bytes(*a, lr_shrink_plan(a->T, a->K, a->max_pieces, a->n_adapters));
+  return lr_t_bytes(*a, lr_shrink_plan(a->T, a->K, a->max_pieces, a->n_adapters)) + lr_list_bytes(*a);
 }
 
 extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeLoraArgs* args, void* stream) {
@@ -522,8 +881,9 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
                   "moe_lora_matmul: adapters must be 16-byte aligned, their rows padded to 8 values");
     MOE_CHECK_ARG(a.ld_x >= (a.K + 7) / 8 * 8, "moe_lora_matmul: rows of x must be padded to 8 values");
     sp = lr_shrink_plan(a.T, a.K, a.max_pieces, a.n_adapters);
-    MOE_CHECK_ARG(a.workspace && (uintptr_t)a.workspace % 256 == 0 && a.workspace_bytes >= lr_t_bytes(a, sp),
-                  "moe_lora_matmul: needs a 256-byte aligned workspace of %zu bytes", lr_t_bytes(a, sp));
+    const size_t need = lr_t_bytes(a, sp) + lr_list_bytes(a);
+    MOE_CHECK_ARG(a.workspace && (uintptr_t)a.workspace % 256 == 0 && a.workspace_bytes >= need,
+                  "moe_lora_matmul: needs a 256-byte aligned workspace of %zu bytes", need);
   }
   cudaStream_t st = (cudaStream_t)stream;
   LoraParams p = {};
@@ -535,7 +895,14 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
     p.t = (float*)a.workspace; p.ld_t = (int64_t)a.max_pieces * LR_PIECE; p.t_parts = sp.parts; p.t_part_stride = a.T * p.ld_t;
   }
   p.y = a.y; p.ld_y = a.ld_y; p.status = a.status;
+  const bool many = lr_many(a.T);
+  const PairPlan pl = many ? lr_pair_plan(a.T, a.K, a.N) : PairPlan{};
+  if (adapters && many) {
+    p.list = (int32_t*)((uint8_t*)a.workspace + lr_t_bytes(a, sp));
+    p.list_tb = pl.tb;
+  }
   if (adapters)
     if (int rc = a.dtype == MOE_F16 ? lr_shrink<__half>(p, sp, st) : lr_shrink<__nv_bfloat16>(p, sp, st)) return rc;
+  if (many) return a.dtype == MOE_F16 ? lr_pair<__half>(p, a, pl, st) : lr_pair<__nv_bfloat16>(p, a, pl, st);
   return a.dtype == MOE_F16 ? lr_stream<__half>(p, a, st) : lr_stream<__nv_bfloat16>(p, a, st);
 }

@@ -133,6 +133,10 @@ _STATUS_TEXT = {
     1101: "projection with adapters: the producer waited for a free piece", 1102: "projection with adapters: the producer waited for a free stage",
     1103: "projection with adapters: the MMA warp waited for a stage", 1104: "projection with adapters: the MMA warp waited for a piece",
     1105: "projection with adapters: the epilogue waited for the accumulator", 1106: "projection with adapters: a writer waited for a free piece",
+    1111: "projection with adapters, pairs: the producer waited for a free stage", 1112: "projection with adapters, pairs: the producer waited for a free piece",
+    1113: "projection with adapters, pairs: the MMA warp waited for a free accumulator", 1114: "projection with adapters, pairs: the MMA warp waited for a stage",
+    1115: "projection with adapters, pairs: the MMA warp waited for a piece", 1116: "projection with adapters, pairs: the epilogue waited for the accumulator",
+    1117: "projection with adapters, pairs: a writer waited for a free piece", 1118: "projection with adapters, pairs: a writer waited for a piece's tile",
 }
 
 
