@@ -9,8 +9,8 @@
 //  2. the product: W's tiles and x's through a ring by TMA, tcgen05.mma.kind::f16 into fp32 in tensor memory; then, into the same accumulator, one MMA per
 //     piece and term: B's tile times the tokens' t, zero for the tokens of other adapters, so that a block of tokens may hold any mixture.  t enters in two
 //     terms (hi + lo, 16 bits of it in bf16), so it costs the result nothing.
-// The second has two forms: lora_stream_kernel for few tokens (weight rows are the MMA's 128 rows, up to 256 tokens its columns, K cut over a cluster) and
-// lora_pair_kernel for many (a pair of SMs per tile of 256 tokens x 256 outputs).
+// The second has two forms: lora_stream_kernel for few tokens, whose adapters' part runs on CUDA cores beside the product, and lora_pair_kernel for many, as
+// above.
 #include "gemm_pair_common.cuh"
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -54,8 +54,8 @@ __device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, i
   }
   __syncthreads();
   for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {          // an adapter counts at its first token
-    bool fresh = idx[r] >= 0;
-    for (int i = 0; i < r && fresh; ++i) fresh = idx[i] != idx[r];
+    bool fresh = idx[r] >= 0 && (r == 0 || idx[r - 1] != idx[r]);        // (most often runs)
+    for (int i = 0; i + 1 < r && fresh; ++i) fresh = idx[i] != idx[r];
     list[r] = fresh ? idx[r] : -1;
   }
   __syncthreads();
@@ -75,13 +75,25 @@ __device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, i
 
 constexpr int SH_WARPS = 8;
 
-// grid: (blocks of 8 NB tokens, pieces of an adapter, shares of k x list places)
+// grid: (blocks of 8 NB tokens, pieces of an adapter and one for the lists, shares of k x list places)
 template <typename T16, int NB>
-__global__ void __launch_bounds__(SH_WARPS * 32) lora_shrink_kernel(const LoraParams p, const int places) {
+__global__ void __launch_bounds__(SH_WARPS * 32, 2) lora_shrink_kernel(const LoraParams p, const int places) {
   __shared__ int s_idx[8 * NB], s_list[8 * NB], s_count;
   __shared__ __align__(16) float s_sum[SH_WARPS][NB][32][4];
   pdl_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qrow = lane >> 2, c4 = lane & 3;
+  if ((int)blockIdx.y == p.max_pieces) {
+    // the adapters of the product's blocks of tokens, for its kernel
+    if (blockIdx.z == 0 && (int64_t)blockIdx.x * p.list_tb < p.T) {
+      int* idx = reinterpret_cast<int*>(s_sum);
+      const int64_t from = (int64_t)blockIdx.x * p.list_tb;
+      adapters_of(p, from, (int)min((int64_t)p.list_tb, (int64_t)p.T - from), p.list_tb, idx, idx + LR_MAX_TB, &s_count);
+      int32_t* out = p.list + (int64_t)blockIdx.x * LR_LIST;
+      for (int i = threadIdx.x; i < s_count; i += SH_WARPS * 32) out[1 + i] = idx[LR_MAX_TB + i];
+      if (threadIdx.x == 0) out[0] = s_count;
+    }
+    return;
+  }
   const int64_t row0 = (int64_t)blockIdx.x * (8 * NB);
   const int rows = (int)min((int64_t)(8 * NB), (int64_t)p.T - row0);
   const int place = blockIdx.z % places, part = blockIdx.z / places;
@@ -138,16 +150,6 @@ __global__ void __launch_bounds__(SH_WARPS * 32) lora_shrink_kernel(const LoraPa
     }
     __syncthreads();
   }
-  // the adapters of the product's blocks of tokens, for its kernel
-  if (p.list_tb > 0 && blockIdx.y == 0 && blockIdx.z == 0 && (int64_t)blockIdx.x * p.list_tb < p.T) {
-    int* idx = reinterpret_cast<int*>(s_sum);
-    const int64_t first = (int64_t)blockIdx.x * p.list_tb;
-    __syncthreads();
-    adapters_of(p, first, (int)min((int64_t)p.list_tb, (int64_t)p.T - first), p.list_tb, idx, idx + LR_MAX_TB, &s_count);
-    int32_t* out = p.list + (int64_t)blockIdx.x * LR_LIST;
-    for (int i = threadIdx.x; i < s_count; i += SH_WARPS * 32) out[1 + i] = idx[LR_MAX_TB + i];
-    if (threadIdx.x == 0) out[0] = s_count;
-  }
 }
 static_assert(2 * LR_MAX_TB * sizeof(int) <= SH_WARPS * 32 * 4 * sizeof(float), "lists in place of the sums");
 
@@ -159,15 +161,6 @@ __device__ __forceinline__ uint32_t piece_desc(uint32_t at) { return PIECE_DESC_
 constexpr uint32_t PIECE_DESC_HI = (256u >> 4) | (1u << 14);            // stride byte offset: between groups of eight rows; sm_100, no swizzle
 __device__ __forceinline__ uint32_t lr_idesc(bool f16, int m, int n) {
   return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void elect_mma_piece(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
-      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PIECE_DESC_HI)
-      : "memory");
 }
 template <typename T16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
   T16 h[2] = {from_f32<T16>(a), from_f32<T16>(b)};
@@ -210,37 +203,84 @@ __device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, 
   sts128(to + lo + 128, l[1]);
 }
 
+// The shares of k of a cluster's CTAs meet, in their order: sums [token][128 outputs] at `at` in the shared memory of the CTAs step * r + base, r < S.  Tokens
+// t0 .. t1 of the block for outputs n0 on; four outputs a thread, four of those on their way at a time.
+template <typename T16>
+__device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, int S, uint32_t step, uint32_t base, int64_t row0, int t0, int t1, int n0) {
+  const bool vec = p.N % 4 == 0 && p.ld_y % 4 == 0 && ((uintptr_t)p.y & 7u) == 0;
+  for (int i0 = threadIdx.x; i0 < (t1 - t0) * 32; i0 += 4 * blockDim.x) {
+    float v[4][4] = {};
+    for (int r = 0; r < S; ++r) {
+      uint32_t from;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(step * (uint32_t)r + base));
+      float q[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(i0 + u * (int)blockDim.x, (t1 - t0) * 32 - 1);
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q[u][0]), "=f"(q[u][1]), "=f"(q[u][2]), "=f"(q[u][3])
+                     : "r"(from + (uint32_t)((t0 + (i >> 5)) * LR_TILE_N + (i & 31) * 4) * 4u) : "memory");
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][j] += q[u][j];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * (int)blockDim.x, n = n0 + (i & 31) * 4;
+      if (i >= (t1 - t0) * 32 || n >= p.N) continue;
+      T16* y = (T16*)p.y + (row0 + t0 + (i >> 5)) * p.ld_y + n;
+      T16 o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (p.bias && n + j < p.N) v[u][j] += load_bias(p.bias, p.bias_dtype, n + j);
+        o[j] = from_f32<T16>(v[u][j]);
+      }
+      if (vec) {
+        *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) y[j] = o[j];
+      }
+    }
+  }
+}
+
 // ---- few tokens ------------------------------------------------------------------------------------------------
-constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-5 epilogue, 6-9 write the tokens' side of the pieces
-constexpr int LS_MAX_STAGES = 8, LS_MAX_PIECES = 4, LS_MAX_TB = 64;
+constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-5 epilogue, 6-9 adapters
+constexpr int LS_MAX_STAGES = 8, LS_MAX_TB = 64;
 
-struct StreamPlan { int tb, splits, stages, pieces, smem; };      // tokens of a block, cluster, ring of k steps, ring of pieces, bytes
+struct StreamPlan { int tb, splits, stages, smem; };           // tokens of a block, cluster, ring of k steps, bytes
 
+__device__ __forceinline__ void adapter_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Single tokens have an adapter each, and an MMA for one of them in 64 columns would be 63 parts zeros that somebody writes: here the second product is
+// made on CUDA cores beside the first.  A thread has an output; 16 ranks of it are 32 bytes of B.
 template <typename T16>
 __global__ void __launch_bounds__(LS_THREADS, 2)
 lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
-  __shared__ __align__(8) uint64_t bars[2 * LS_MAX_STAGES + 2 * LS_MAX_PIECES + 1];
+  __shared__ __align__(8) uint64_t bars[2 * LS_MAX_STAGES + 1];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_count;
-  __shared__ int s_idx[LS_MAX_TB], s_list[LS_MAX_TB], s_first[LS_MAX_TB], s_np[LS_MAX_TB];
+  __shared__ int s_abort;
+  __shared__ int s_idx[LS_MAX_TB], s_first[LS_MAX_TB], s_from[LS_MAX_TB], s_count;
+  __shared__ unsigned long long s_mask[LS_MAX_TB];             // the tokens of an adapter
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int TB = pl.tb;
-  const uint32_t X_BYTES = (uint32_t)TB * 128u, stage_bytes = SUBTILE_BYTES + X_BYTES, T_BYTES = (uint32_t)TB * 32u, piece_bytes = LR_PIECE_BYTES + 2 * T_BYTES;
-  const uint32_t piece0 = sbase + (uint32_t)pl.stages * stage_bytes;
+  const uint32_t X_BYTES = (uint32_t)TB * 128u, stage_bytes = SUBTILE_BYTES + X_BYTES;
+  float* part = reinterpret_cast<float*>(smem);                // [token][output], over the ring once the product is done
+  float* extra = reinterpret_cast<float*>(smem + pl.stages * stage_bytes);      // the same of the adapters
   auto FULL = [&](int s) { return smem_u32(&bars[s]); };
   auto EMPTY = [&](int s) { return smem_u32(&bars[LS_MAX_STAGES + s]); };
-  auto PFULL = [&](int s) { return smem_u32(&bars[2 * LS_MAX_STAGES + s]); };
-  auto PEMPTY = [&](int s) { return smem_u32(&bars[2 * LS_MAX_STAGES + LS_MAX_PIECES + s]); };
-  const uint32_t ACC = smem_u32(&bars[2 * LS_MAX_STAGES + 2 * LS_MAX_PIECES]);
+  const uint32_t ACC = smem_u32(&bars[2 * LS_MAX_STAGES]);
   const Ctl ctl{&s_abort, p.status};
-  const uint32_t tmem_cols = TB <= 32 ? 32u : TB <= 64 ? 64u : TB <= 128 ? 128u : 256u;
+  const uint32_t tmem_cols = TB <= 32 ? 32u : 64u;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < LS_MAX_STAGES; ++s) { mbar_init(FULL(s), 1); mbar_init(EMPTY(s), 1); }
-    for (int s = 0; s < LS_MAX_PIECES; ++s) { mbar_init(PFULL(s), 2); mbar_init(PEMPTY(s), 1); }
     mbar_init(ACC, 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -262,52 +302,24 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
   const int n0 = blockIdx.x * LR_TILE_N, rank = blockIdx.z, S = pl.splits;
   const int64_t row0 = (int64_t)blockIdx.y * TB;
   const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0);
-  adapters_of(p, row0, rows, TB, s_idx, s_list, &s_count);
-  const int n_list = s_count;
-  for (int i = threadIdx.x; i < n_list; i += LS_THREADS) {
-    s_first[i] = p.first[s_list[i]];
-    s_np[i] = p.first[s_list[i] + 1] - s_first[i];
-  }
-  __syncthreads();
   const int KT = (p.K + BLOCK_K - 1) / BLOCK_K, kt0 = KT * rank / S, kt1 = KT * (rank + 1) / S;
-  // the pieces of this CTA, every S-th of the block's: calls f(number, place in the list, piece of that adapter)
-  auto pieces = [&](auto f) {
-    int g = 0, mine = 0;
-    for (int l = 0; l < n_list; ++l)
-      for (int i = 0; i < s_np[l]; ++i, ++g)
-        if (g % S == rank && !f(mine++, l, i)) return;
-  };
 
   if (warp == 0) {
     // ================================= producer ================================================================
-    int it = 0, issued = 0;
+    int it = 0;
     bool ok = true;
-    auto piece = [&](int m, int l, int i) {
-      const int s = m % pl.pieces;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1101));
-      if (!ok) return false;
-      elect_expect_tx(PFULL(s), LR_PIECE_BYTES);
-      if (lane == 0) bulk_g2s(piece0 + (uint32_t)s * piece_bytes, p.b + ((int64_t)(s_first[l] + i) * p.NP + n0) * 32, LR_PIECE_BYTES, PFULL(s));
-      ++issued;
-      return true;
-    };
-    pieces([&](int m, int l, int i) { return m < pl.pieces && piece(m, l, i); });      // as many as the ring holds, ahead of the product
-    const int ahead = issued;
     for (int kt = kt0; kt < kt1 && ok; ++kt, ++it) {
       const int s = it % pl.stages;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(s), ((it / pl.stages) & 1u) ^ 1u, ctl, 1102));
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(s), ((it / pl.stages) & 1u) ^ 1u, ctl, 1101));
       if (!ok) break;
       const uint32_t st = sbase + (uint32_t)s * stage_bytes;
       elect_expect_tx(FULL(s), stage_bytes);
       elect_tile_2d(st, &w_map, kt * BLOCK_K, n0, FULL(s));
       elect_tile_2d(st + SUBTILE_BYTES, &x_map, kt * BLOCK_K, (int)row0, FULL(s));
     }
-    if (ok) pieces([&](int m, int l, int i) { return m < ahead || piece(m, l, i); });
-    if (!ok && lane == 0) {                                   // copies in flight land before the block's shared memory goes
+    if (!ok && lane == 0)                                     // copies in flight land before the block's shared memory goes
       for (int j = it > pl.stages ? it - pl.stages : 0; j < it; ++j)
         for (uint32_t w = 0; w < (1u << 16) && !mbar_test(FULL(j % pl.stages), (j / pl.stages) & 1u); ++w) __nanosleep(64);
-      __nanosleep(100000);                                    // (a piece's barrier also waits for its writer)
-    }
     __syncwarp();
   } else if (warp == 1) {
     // ================================= MMA =====================================================================
@@ -316,38 +328,24 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     const uint32_t idesc = lr_idesc(std::is_same<T16, __half>::value, 128, TB);
     for (int kt = kt0; kt < kt1; ++kt, ++it) {
       const int s = it % pl.stages;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(FULL(s), (it / pl.stages) & 1u, ctl, 1103));
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(FULL(s), (it / pl.stages) & 1u, ctl, 1102));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t st = sbase + (uint32_t)s * stage_bytes;
-      const uint32_t a_lo = DESC_LO | ((st & 0x3FFFFu) >> 4), b_lo = DESC_LO | (((st + SUBTILE_BYTES) & 0x3FFFFu) >> 4);
+      const uint32_t st = (sbase + (uint32_t)s * stage_bytes) & 0x3FFFFu;
+      const uint32_t a_lo = DESC_LO | (st >> 4), b_lo = DESC_LO | ((st + SUBTILE_BYTES) >> 4);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) elect_mma_bf16(tmem, a_lo + kk * 2, b_lo + kk * 2, idesc, (it | kk) ? 1u : 0u);
       elect_commit(EMPTY(s));
     }
-    if (ok)
-      pieces([&](int m, int, int) {
-        const int s = m % pl.pieces;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(PFULL(s), (m / pl.pieces) & 1u, ctl, 1104));
-        if (!ok) return false;
-        tc_fence_after();
-        const uint32_t st = piece0 + (uint32_t)s * piece_bytes;
-        const uint32_t a_lo = piece_desc(st), b_lo = piece_desc(st + LR_PIECE_BYTES);
-        elect_mma_piece(tmem, a_lo, b_lo, idesc, (it | m) ? 1u : 0u);
-        elect_mma_piece(tmem, a_lo, b_lo + (T_BYTES >> 4), idesc, 1u);
-        elect_commit(PEMPTY(s));
-        return true;
-      });
     elect_commit(ACC);
     if (!ok)
       for (uint32_t w = 0; w < (1u << 16) && !mbar_test(ACC, 0); ++w) __nanosleep(64);
     __syncwarp();
   } else if (warp < 6) {
-    // ================================= accumulator to shared memory: [token][output], over the ring ==================
-    if (__all_sync(0xFFFFFFFFu, mbar_wait(ACC, 0, ctl, 1105))) {
+    // ================================= accumulator to shared memory ==================================================
+    if (__all_sync(0xFFFFFFFFu, mbar_wait(ACC, 0, ctl, 1103))) {
       tc_fence_after();
       const int qd = warp & 3;
-      float* part = reinterpret_cast<float*>(smem);
       for (int c0 = 0; c0 < TB; c0 += 16) {
         uint32_t v[16];
         tmem_ld16(tmem + (uint32_t)c0 + ((uint32_t)(qd * 32) << 16), v);
@@ -358,43 +356,131 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     }
     tc_fence_before();
   } else {
-    // ================================= tokens' side of the pieces ===================================================
-    pieces([&](int m, int l, int i) {
-      const int s = m % pl.pieces;
-      if (s != warp - 6) return true;                         // a warp has a place of the ring: it sees every phase of its barrier
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1106))) return false;
-      const uint32_t dst = piece0 + (uint32_t)s * piece_bytes + LR_PIECE_BYTES;
-      for (int r = lane; r < TB; r += 32) write_piece_row<T16>(p, s_idx[r] == s_list[l], row0 + r, i * LR_PIECE, dst, T_BYTES, r);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(PFULL(s));
+    // ================================= adapters ================================================================
+    const int tid = threadIdx.x - 192;                        // output n0 + tid
+    for (int t = 0; t < TB; ++t) extra[t * LR_TILE_N + tid] = 0.0f;
+    if (tid < TB) {
+      const int a = tid < rows && p.indx ? p.indx[row0 + tid] : -1;
+      s_idx[tid] = a >= 0 && a < p.n_adapters ? a : -1;
+    }
+    adapter_bar();
+    // an adapter counts at its first token: its tokens and its pieces, the pieces numbered through
+    if (warp == 6) {
+      int run = 0;
+      for (int t0 = 0; t0 < TB; t0 += 32) {
+        const int t = t0 + lane, a = t < TB ? s_idx[t] : -1;
+        unsigned long long mask = 0;
+        if (a >= 0)
+          for (int i = 0; i < TB; ++i) mask |= (unsigned long long)(s_idx[i] == a) << i;
+        const bool fresh = mask != 0 && __ffsll((long long)mask) - 1 == t;
+        const int f = fresh ? p.first[a] : 0, np = fresh ? p.first[a + 1] - f : 0;
+        int sum = np;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int q = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+          if (lane >= o) sum += q;
+        }
+        if (t < TB) {
+          s_mask[t] = mask;
+          s_first[t] = f;
+          s_from[t] = run + sum - np;                         // (of tokens that are not the first of their adapter: no pieces)
+        }
+        run += __shfl_sync(0xFFFFFFFFu, sum, 31);
+      }
+      if (lane == 0) s_count = run;
+    }
+    adapter_bar();
+    // every S-th piece is this CTA's, with each of its adapter's tokens
+    const uint8_t* b = p.b + (int64_t)(n0 >> 3) * 256;
+    const int n_mine = s_count > rank ? (s_count - rank + S - 1) / S : 0;
+    // -> the list place of this CTA's j-th piece, and which of that adapter's pieces it is
+    auto find = [&](int j, int& l, int& i) {
+      const int g = rank + S * j;
+      int lo = 0, hi = TB;                                    // the last place that starts at or before g is the one with pieces
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_from[mid] <= g) lo = mid; else hi = mid;
+      }
+      l = lo;
+      i = g - s_from[lo];
+    };
+    for (int j = tid; j < n_mine; j += 128) {
+      int l, i;
+      find(j, l, i);
+      l2_hint(b + (int64_t)(s_first[l] + i) * p.NP * 32, LR_PIECE_BYTES);
+    }
+    b += (tid >> 3) * 256 + (tid & 7) * 16;
+    int j = -1, my_l = 0, my_i = 0, l = 0, i = 0, t = 0;      // a lane knows one piece of every 32
+    unsigned long long mask = 0;
+    auto advance = [&]() {                                    // to the next token of a piece; false behind the last
+      if (mask == 0) {
+        if (++j >= n_mine) return false;
+        if ((j & 31) == 0 && j + lane < n_mine) find(j + lane, my_l, my_i);
+        l = __shfl_sync(0xFFFFFFFFu, my_l, j & 31);
+        i = __shfl_sync(0xFFFFFFFFu, my_i, j & 31);
+        mask = s_mask[l];
+      }
+      t = __ffsll((long long)mask) - 1;
+      mask &= mask - 1;
       return true;
-    });
-  }
-  __syncthreads();
-  auto cluster_barrier = []() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
-  if (S > 1) cluster_barrier();
-  // ---- the cluster's shares of k meet, in their order: each CTA takes a share of the tokens ----
-  bool ok = true;
-  auto remote = [&](uint32_t at, int r) {
-    uint32_t v;
-    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(at), "r"(r) : "memory");
-    return v;
-  };
-  for (int r = 0; r < S; ++r) ok = ok && (S > 1 ? remote(smem_u32(&s_abort), r) : (uint32_t)s_abort) == 0;
-  if (ok) {
-    const int t0 = rows * rank / S, t1 = rows * (rank + 1) / S;
-    for (int i = threadIdx.x; i < (t1 - t0) * LR_TILE_N; i += LS_THREADS) {
-      const int tok = t0 + (i >> 7), n = n0 + (i & 127);
-      if (n >= p.N) continue;
-      const uint32_t at = sbase + (uint32_t)(tok * LR_TILE_N + (i & 127)) * 4u;
-      float v = 0.0f;
-      for (int r = 0; r < S; ++r) v += __uint_as_float(S > 1 ? remote(at, r) : lds32(at));
-      if (p.bias) v += load_bias(p.bias, p.bias_dtype, n);
-      ((T16*)p.y)[(row0 + tok) * p.ld_y + n] = from_f32<T16>(v);
+    };
+    const float* ranks = p.t + row0 * p.ld_t + (lane & 15);   // a lane holds one of the sixteen ranks of a token
+    bool more = advance();
+    while (more) {
+      constexpr int U = 4;                                    // everything of four pairs is asked for before the first is taken on
+      uint4 w[U][2];
+      float r[U][4];
+      int at[U], rest[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        at[u] = -1;
+        rest[u] = 0;
+        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[u][q] = 0.0f;
+        if (more) {
+          const uint4* src = reinterpret_cast<const uint4*>(b + (int64_t)(s_first[l] + i) * p.NP * 32);
+          w[u][0] = src[0];
+          w[u][1] = src[8];
+          at[u] = t;
+          rest[u] = t * (int)p.ld_t + i * LR_PIECE;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < p.t_parts) r[u][q] = ranks[q * p.t_part_stride + rest[u]];
+          more = advance();
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (at[u] < 0) break;
+        float mine = (r[u][0] + r[u][1]) + (r[u][2] + r[u][3]);
+        for (int q = 4; q < p.t_parts; ++q) mine += ranks[q * p.t_part_stride + rest[u]];
+        const T16* e = reinterpret_cast<const T16*>(&w[u][0]);
+        float v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v = fmaf(__shfl_sync(0xFFFFFFFFu, mine, j), to_f32<T16>(e[j]), v);
+        extra[at[u] * LR_TILE_N + tid] += v;
+      }
     }
   }
-  if (S > 1) cluster_barrier();                               // no CTA leaves while its sums are read
+  __syncthreads();
+  // the adapters' share on top of the product's
+  for (int i = threadIdx.x; i < rows * 32; i += LS_THREADS) {
+    float4 v = reinterpret_cast<float4*>(part)[i];
+    const float4 e = reinterpret_cast<const float4*>(extra)[i];
+    v.x += e.x; v.y += e.y; v.z += e.z; v.w += e.w;
+    reinterpret_cast<float4*>(part)[i] = v;
+  }
+  __syncthreads();
+  if (S > 1) cluster_sync_all();
+  bool ok = true;
+  for (int r = 0; r < S; ++r) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(smem_u32(&s_abort)), "r"(r) : "memory");
+    ok = ok && v == 0;
+  }
+  if (ok) cluster_sums<T16>(p, sbase, S, 1u, 0u, row0, rows * rank / S, rows * (rank + 1) / S, n0);
+  if (S > 1) cluster_sync_all();                              // no CTA leaves while its sums are read
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
@@ -640,16 +726,8 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
     if (ok && tile0 < tile1) {
       const int block = tile0 / pl.tiles_n, n0 = (tile0 - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
       const int64_t row0 = (int64_t)block * TB;
-      const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0), t0 = rows * split / S, t1 = rows * (split + 1) / S;
-      for (int i = threadIdx.x; i < (t1 - t0) * LR_TILE_N; i += LP_THREADS) {
-        const int tok = t0 + (i >> 7), n = n0 + (i & 127);
-        if (n >= p.N) continue;
-        const uint32_t at = sbase + (uint32_t)(tok * LR_TILE_N + (i & 127)) * 4u;
-        float v = 0.0f;
-        for (int r = 0; r < S; ++r) v += __uint_as_float(remote(at, (uint32_t)(2 * r) + half_id));
-        if (p.bias) v += load_bias(p.bias, p.bias_dtype, n);
-        ((T16*)p.y)[(row0 + tok) * p.ld_y + n] = from_f32<T16>(v);
-      }
+      const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0);
+      cluster_sums<T16>(p, sbase, S, 2u, half_id, row0, rows * split / S, rows * (split + 1) / S, n0);
     }
     cluster_sync_all();                                       // no CTA leaves while its sums are read
   }
@@ -697,11 +775,12 @@ ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   s.nb = T <= 128 ? 1 : 8;
   const int64_t blocks = cdiv64(T, 8 * s.nb);
   const int64_t most = n_adapters < 8 * s.nb ? n_adapters : 8 * s.nb;             // adapters that a block can hold
-  s.places = (int)(most < (s.nb == 1 ? 8 : 4) ? most : (s.nb == 1 ? 8 : 4));
-  if (s.places < 1) s.places = 1;
-  // shares of k while there are fewer CTAs than SMs
+  const int64_t want = s.nb == 1 ? 8 : T <= 1024 ? 16 : 4;      // (a place without an adapter costs a block of threads all the same)
+  s.places = (int)(most < want ? most : want);
+  // shares of k up to as many blocks with something to do as there are SMs, twice as many of the long ones
+  const int64_t enough = moe_sm_count() * (s.nb == 1 ? 1 : 2);
   int parts = 1;
-  while (parts < 8 && blocks * max_pieces * s.places * parts * 2 <= moe_sm_count() && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
+  while (parts < 8 && blocks * max_pieces * parts * 2 <= enough && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
   s.parts = parts;
   return s;
 }
@@ -710,18 +789,15 @@ StreamPlan lr_stream_plan(int64_t T, int K, int N) {
   StreamPlan pl;
   pl.tb = T >= LS_MAX_TB ? LS_MAX_TB : (int)cdiv64(T, 16) * 16;
   const int64_t tiles = cdiv64(N, LR_TILE_N) * cdiv64(T, pl.tb), KT = cdiv64(K, BLOCK_K);
-  const int stage = SUBTILE_BYTES + pl.tb * 128, piece = LR_PIECE_BYTES + pl.tb * 64;
+  const int stage = SUBTILE_BYTES + pl.tb * 128, sums = pl.tb * LR_TILE_N * 4;
   // Two CTAs per SM.  k is cut as long as the clusters fit side by side, which they do not up to the last place: 40 tiles took 21.5 us in clusters of four
   // to six CTAs and 29.7 in clusters of seven (280 CTAs of 296), where some wait for a second round.
   int64_t s = moe_sm_count() * 5 / 3 / tiles;
   if (s > KT / 4) s = KT / 4;
   pl.splits = (int)(s < 1 ? 1 : s > 6 ? 6 : s);
-  pl.pieces = LS_MAX_PIECES;
-  const int st = (104 * 1024 - pl.pieces * piece) / stage;
+  const int st = (104 * 1024 - sums) / stage;
   pl.stages = st > LS_MAX_STAGES ? LS_MAX_STAGES : st;
-  int bytes = pl.stages * stage + pl.pieces * piece;
-  if (bytes < pl.tb * LR_TILE_N * 4) bytes = pl.tb * LR_TILE_N * 4;
-  pl.smem = bytes + 1024;
+  pl.smem = pl.stages * stage + sums + 1024;                  // (the product's sums take the ring's place: two stages are enough for them)
   return pl;
 }
 
@@ -805,7 +881,7 @@ int lr_check(const MoeLoraArgs* a) {
 }
 
 template <typename T16> int lr_shrink(const LoraParams& p, const ShrinkPlan& sp, cudaStream_t st) {
-  const dim3 grid((unsigned)cdiv64(p.T, 8 * sp.nb), (unsigned)p.max_pieces, (unsigned)(sp.places * sp.parts));
+  const dim3 grid((unsigned)cdiv64(p.T, 8 * sp.nb), (unsigned)(p.max_pieces + (p.list_tb > 0 ? 1 : 0)), (unsigned)(sp.places * sp.parts));
   if (sp.nb == 1) MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 1>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
   else MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 8>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
   MOE_CHECK_LAUNCH();

@@ -130,9 +130,8 @@ _STATUS_TEXT = {
     1001: "layer of a few tokens: the weight producer waited for a free stage", 1002: "layer of a few tokens: a warp waited for weights",
     1003: "layer of a few tokens: fc2 waited for fc1's rows", 1004: "layer of a few tokens: the combine waited for fc2's sums",
     1005: "layer of a few tokens: the epilogue waited for a unit's sums", 1006: "layer of a few tokens: a warp waited for a free buffer of sums",
-    1101: "projection with adapters: the producer waited for a free piece", 1102: "projection with adapters: the producer waited for a free stage",
-    1103: "projection with adapters: the MMA warp waited for a stage", 1104: "projection with adapters: the MMA warp waited for a piece",
-    1105: "projection with adapters: the epilogue waited for the accumulator", 1106: "projection with adapters: a writer waited for a free piece",
+    1101: "projection with adapters: the producer waited for a free stage", 1102: "projection with adapters: the MMA warp waited for a stage",
+    1103: "projection with adapters: the epilogue waited for the accumulator",
     1111: "projection with adapters, pairs: the producer waited for a free stage", 1112: "projection with adapters, pairs: the producer waited for a free piece",
     1113: "projection with adapters, pairs: the MMA warp waited for a free accumulator", 1114: "projection with adapters, pairs: the MMA warp waited for a stage",
     1115: "projection with adapters, pairs: the MMA warp waited for a piece", 1116: "projection with adapters, pairs: the epilogue waited for the accumulator",
