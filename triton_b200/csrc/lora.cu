@@ -30,7 +30,7 @@ struct LoraParams {
   const int32_t* indx;
   float* t; int64_t ld_t; int t_parts; int64_t t_part_stride;     // shares of k whose sums make up t
   void* y; int64_t ld_y;
-  int32_t* list; int list_tb;                          // the adapters of every block of list_tb tokens: [LR_LIST] their count, then they
+  int32_t* list; int list_tb;                          // of every block of list_tb tokens [LR_LIST]: how many adapters, how many pieces, the adapters
   int32_t* status;
 };
 constexpr int LR_MAX_TB = 512, LR_LIST = LR_MAX_TB + 4;
@@ -46,7 +46,8 @@ template <typename T16> __device__ __forceinline__ void mma_16816(float (&d)[4],
 }
 
 // Adapter of each of `rows` tokens from row0 on (-1: none, and for the rows past them) and the list of those that occur, in the order of their first
-// token.  All threads of the block call; `idx` and `list` are in shared memory; behind a barrier, with one at the end.
+// token.  All threads of the block call; `idx` (16-byte aligned) and `list`, block_rows (a multiple of 4) each, are in shared memory; behind a
+// barrier, with one at the end.
 __device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, int rows, int block_rows, int* idx, int* list, int* count) {
   for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {
     const int a = r < rows && p.indx ? p.indx[row0 + r] : -1;
@@ -55,7 +56,16 @@ __device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, i
   __syncthreads();
   for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {          // an adapter counts at its first token
     bool fresh = idx[r] >= 0 && (r == 0 || idx[r - 1] != idx[r]);        // (most often runs)
-    for (int i = 0; i + 1 < r && fresh; ++i) fresh = idx[i] != idx[r];
+    for (int i = 0; i < r && fresh; i += 16) {                // (behind r up to the next multiple of 16, all of the block's)
+      int same = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (i + 4 * q >= block_rows) break;
+        const int4 v = *reinterpret_cast<const int4*>(idx + i + 4 * q);
+        same |= (v.x == idx[r] && i + 4 * q < r) | (v.y == idx[r] && i + 4 * q + 1 < r) | (v.z == idx[r] && i + 4 * q + 2 < r) | (v.w == idx[r] && i + 4 * q + 3 < r);
+      }
+      fresh = !same;
+    }
     list[r] = fresh ? idx[r] : -1;
   }
   __syncthreads();
@@ -75,10 +85,12 @@ __device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, i
 
 constexpr int SH_WARPS = 8;
 
-// grid: (blocks of 8 NB tokens, pieces of an adapter and one for the lists, shares of k x list places)
+// grid: (blocks of 8 NB tokens, pieces of an adapter and one for the lists, shares of k x places in the list of the block's adapters).  A block of
+// threads has one adapter of its tokens (eights), or every `places`-th (sixty-fours), and splits k over its warps: what it takes is one or two trips to
+// memory, and a warp with an adapter to itself took four times as many.
 template <typename T16, int NB>
-__global__ void __launch_bounds__(SH_WARPS * 32, 2) lora_shrink_kernel(const LoraParams p, const int places) {
-  __shared__ int s_idx[8 * NB], s_list[8 * NB], s_count;
+__global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_kernel(const LoraParams p, const int places) {
+  __shared__ __align__(16) int s_idx[8 * NB], s_list[8 * NB], s_count;
   __shared__ __align__(16) float s_sum[SH_WARPS][NB][32][4];
   pdl_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qrow = lane >> 2, c4 = lane & 3;
@@ -89,18 +101,44 @@ __global__ void __launch_bounds__(SH_WARPS * 32, 2) lora_shrink_kernel(const Lor
       const int64_t from = (int64_t)blockIdx.x * p.list_tb;
       adapters_of(p, from, (int)min((int64_t)p.list_tb, (int64_t)p.T - from), p.list_tb, idx, idx + LR_MAX_TB, &s_count);
       int32_t* out = p.list + (int64_t)blockIdx.x * LR_LIST;
-      for (int i = threadIdx.x; i < s_count; i += SH_WARPS * 32) out[1 + i] = idx[LR_MAX_TB + i];
-      if (threadIdx.x == 0) out[0] = s_count;
+      const int n = s_count;
+      int total = 0;
+      for (int i = threadIdx.x; i < n; i += SH_WARPS * 32) {
+        const int a = idx[LR_MAX_TB + i];
+        out[2 + i] = a;
+        total += p.first[a + 1] - p.first[a];
+      }
+      total = __reduce_add_sync(0xFFFFFFFFu, total);
+      __syncthreads();
+      if (threadIdx.x == 0) s_count = 0;
+      __syncthreads();
+      if (lane == 0) atomicAdd(&s_count, total);
+      __syncthreads();
+      if (threadIdx.x == 0) { out[0] = n; out[1] = s_count; }
     }
     return;
   }
   const int64_t row0 = (int64_t)blockIdx.x * (8 * NB);
   const int rows = (int)min((int64_t)(8 * NB), (int64_t)p.T - row0);
   const int place = blockIdx.z % places, part = blockIdx.z / places;
-  adapters_of(p, row0, rows, 8 * NB, s_idx, s_list, &s_count);
+  int count, only = -1;
+  if constexpr (NB == 1) {                                    // every warp for itself: most blocks of threads find that there is nothing for them
+    int a = lane < rows ? p.indx[row0 + lane] : -1;
+    a = a >= 0 && a < p.n_adapters ? a : -1;
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, a);
+    uint32_t fresh = __ballot_sync(0xFFFFFFFFu, a >= 0 && __ffs(same) - 1 == lane);
+    count = __popc(fresh);
+    if (place >= count) return;
+    for (int i = 0; i < place; ++i) fresh &= fresh - 1;
+    only = __shfl_sync(0xFFFFFFFFu, a, __ffs(fresh) - 1);
+    if (warp == 0 && lane < 8) s_idx[lane] = a;
+  } else {
+    adapters_of(p, row0, rows, 8 * NB, s_idx, s_list, &s_count);
+    count = s_count;
+  }
   const int K8 = (p.K + 7) & ~7, blocks = (K8 + 31) >> 5, b0 = blocks * part / p.t_parts, b1 = blocks * (part + 1) / p.t_parts;
-  for (int l = place; l < s_count; l += places) {
-    const int a = s_list[l], f = p.first[a];
+  for (int l = place; l < count; l += places) {
+    const int a = NB == 1 ? only : s_list[l], f = p.first[a];
     if ((int)blockIdx.y >= p.first[a + 1] - f) continue;      // (uniform)
     const T16* ra = (const T16*)p.a + (int64_t)(f + blockIdx.y) * LR_PIECE * p.ld_a;
     float acc[NB][4];
@@ -135,18 +173,17 @@ __global__ void __launch_bounds__(SH_WARPS * 32, 2) lora_shrink_kernel(const Lor
         }
     }
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s_sum[warp][n][lane][j] = acc[n][j];
+    for (int n = 0; n < NB; ++n) *reinterpret_cast<float4*>(s_sum[warp][n][lane]) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
     __syncthreads();
+    const float scale = p.scale[a];
     for (int i = threadIdx.x; i < NB * 128; i += SH_WARPS * 32) {
-      const int n = i >> 7, token = n * 8 + ((i >> 4) & 7), rank = i & 15;       // accumulator: rank rows, token columns
+      const int n = i >> 7, token = i >> 4, rank = i & 15;    // accumulator: rank rows, token columns
       const int ln = (rank & 7) * 4 + ((token & 7) >> 1), j = (rank >> 3) * 2 + (token & 1);
+      if (s_idx[token] != a) continue;
       float v = 0.0f;
 #pragma unroll
       for (int w = 0; w < SH_WARPS; ++w) v += s_sum[w][n][ln][j];
-      if (s_idx[token] == a)
-        p.t[part * p.t_part_stride + (row0 + token) * p.ld_t + blockIdx.y * LR_PIECE + rank] = v * p.scale[a];
+      p.t[part * p.t_part_stride + (row0 + token) * p.ld_t + blockIdx.y * LR_PIECE + rank] = v * scale;
     }
     __syncthreads();
   }
@@ -203,38 +240,41 @@ __device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, 
   sts128(to + lo + 128, l[1]);
 }
 
-// The shares of k of a cluster's CTAs meet, in their order: sums [token][128 outputs] at `at` in the shared memory of the CTAs step * r + base, r < S.  Tokens
-// t0 .. t1 of the block for outputs n0 on; four outputs a thread, four of those on their way at a time.
-template <typename T16>
+// The shares of k of a cluster's CTAs meet, in their order: sums [token][128 outputs] at `at` in the shared memory of the CTAs step * r + base, r < S <=
+// MOST.  Tokens t0 .. t1 of the block for outputs n0 on; four outputs a thread, U of those and all shares on their way at a time (one share after the other
+// the sums of 300 tokens took 6 us).
+template <typename T16, int MOST, int U>
 __device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, int S, uint32_t step, uint32_t base, int64_t row0, int t0, int t1, int n0) {
   const bool vec = p.N % 4 == 0 && p.ld_y % 4 == 0 && ((uintptr_t)p.y & 7u) == 0;
-  for (int i0 = threadIdx.x; i0 < (t1 - t0) * 32; i0 += 4 * blockDim.x) {
-    float v[4][4] = {};
-    for (int r = 0; r < S; ++r) {
-      uint32_t from;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(step * (uint32_t)r + base));
-      float q[4][4];
+  uint32_t from[MOST];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = min(i0 + u * (int)blockDim.x, (t1 - t0) * 32 - 1);
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q[u][0]), "=f"(q[u][1]), "=f"(q[u][2]), "=f"(q[u][3])
-                     : "r"(from + (uint32_t)((t0 + (i >> 5)) * LR_TILE_N + (i & 31) * 4) * 4u) : "memory");
-      }
+  for (int r = 0; r < MOST; ++r)
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from[r]) : "r"(at), "r"(step * (uint32_t)min(r, S - 1) + base));
+  for (int i0 = threadIdx.x; i0 < (t1 - t0) * 32; i0 += U * blockDim.x) {
+    float q[U][MOST][4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * (int)blockDim.x, (t1 - t0) * 32 - 1);
+      const uint32_t off = (uint32_t)((t0 + (i >> 5)) * LR_TILE_N + (i & 31) * 4) * 4u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[u][j] += q[u][j];
+      for (int r = 0; r < MOST; ++r)
+        if (r < S)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q[u][r][0]), "=f"(q[u][r][1]), "=f"(q[u][r][2]), "=f"(q[u][r][3]) : "r"(from[r] + off) : "memory");
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int i = i0 + u * (int)blockDim.x, n = n0 + (i & 31) * 4;
       if (i >= (t1 - t0) * 32 || n >= p.N) continue;
       T16* y = (T16*)p.y + (row0 + t0 + (i >> 5)) * p.ld_y + n;
       T16 o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (p.bias && n + j < p.N) v[u][j] += load_bias(p.bias, p.bias_dtype, n + j);
-        o[j] = from_f32<T16>(v[u][j]);
+        float v = q[u][0][j];
+#pragma unroll
+        for (int r = 1; r < MOST; ++r)
+          if (r < S) v += q[u][r][j];
+        if (p.bias && n + j < p.N) v += load_bias(p.bias, p.bias_dtype, n + j);
+        o[j] = from_f32<T16>(v);
       }
       if (vec) {
         *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(o);
@@ -249,7 +289,7 @@ __device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, i
 
 // ---- few tokens ------------------------------------------------------------------------------------------------
 constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-5 epilogue, 6-9 adapters
-constexpr int LS_MAX_STAGES = 8, LS_MAX_TB = 64;
+constexpr int LS_MAX_STAGES = 8, LS_MAX_TB = 64, LS_MAX_SPLITS = 6;
 
 struct StreamPlan { int tb, splits, stages, smem; };           // tokens of a block, cluster, ring of k steps, bytes
 
@@ -479,7 +519,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(smem_u32(&s_abort)), "r"(r) : "memory");
     ok = ok && v == 0;
   }
-  if (ok) cluster_sums<T16>(p, sbase, S, 1u, 0u, row0, rows * rank / S, rows * (rank + 1) / S, n0);
+  if (ok) cluster_sums<T16, LS_MAX_SPLITS, 2>(p, sbase, S, 1u, 0u, row0, rows * rank / S, rows * (rank + 1) / S, n0);
   if (S > 1) cluster_sync_all();                              // no CTA leaves while its sums are read
   if (warp == 1) {
     tc_fence_after();
@@ -493,7 +533,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
 // clusters): a k step of 64 brings (128 + tb / 2) rows of 128 bytes into each SM, so the tile is as large as tensor memory, one accumulator
 // at a time, and the ring is filled again while it is drained.  With few tiles k is cut over up to four pairs of a larger cluster, whose sums meet through distributed
 // shared memory as in the kernel above.
-constexpr int LP_THREADS = 320, LP_MAX_STAGES = 4, LP_MAX_PIECES = 4;
+constexpr int LP_THREADS = 320, LP_MAX_STAGES = 4, LP_MAX_PIECES = 4, LP_MAX_SPLITS = 4;
 struct PairPlan { int tb, mmas, splits, stages, pieces, tiles_n, blocks, clusters, smem; };
 
 __device__ __forceinline__ void elect_mma_pair_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
@@ -574,26 +614,11 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
   const int tiles = pl.tiles_n * pl.blocks, me = blockIdx.x / (2 * S);
   // consecutive tiles have the same tokens; one tile per cluster where k is cut
   const int tile0 = (int)((int64_t)tiles * me / pl.clusters), tile1 = (int)((int64_t)tiles * (me + 1) / pl.clusters);
-  // this split's pieces of a token block: calls f(number, adapter, piece of that adapter); `m` runs on over the tiles
-  auto pieces = [&](int block, int& m, auto f) {
-    if (p.list == nullptr) return true;
-    const int32_t* list = p.list + (int64_t)block * LR_LIST;
-    const int n = list[0];
-    int g = 0;
-    for (int l = 0; l < n; ++l) {
-      const int a = list[1 + l], np = p.first[a + 1] - p.first[a];
-      for (int i = 0; i < np; ++i, ++g)
-        if (g % S == split) {
-          if (!f(m, a, i)) return false;
-          ++m;
-        }
-    }
-    return true;
-  };
-
+  // The loops that issue copies and MMAs look at nothing that differs between lanes, as far as the compiler can tell: an operand that it takes from a vector
+  // register, or a loop that it takes for divergent, costs them more than the instruction (with the pieces' list in them, 194 us of 154).
   if (warp == 0) {
     // ================================= producer ================================================================
-    int it = 0, m = 0;
+    int it = 0;
     bool ok = true;
     for (int tile = tile0; tile < tile1 && ok; ++tile) {
       const int block = tile / pl.tiles_n, n0 = (tile - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
@@ -607,15 +632,6 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
         for (int j = 0; j < pl.mmas; ++j)
           elect_tile_pair(st + SUBTILE_BYTES + (uint32_t)(j * half) * 128u, &x_map, kt * BLOCK_K, block * TB + j * n_mma + (int)half_id * half, FULL(s));
       }
-      ok = ok && pieces(block, m, [&](int m, int a, int i) {
-        const int s = m % pl.pieces;
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1112))) return false;
-        elect_expect_tx(PTILE(s), LR_PIECE_BYTES);
-        // (rows of B are padded to 128: the odd CTA of the last tile may have none)
-        const int64_t at = ((int64_t)(p.first[a] + i) * p.NP + (n0 < p.NP ? n0 : 0)) * 32;
-        if (lane == 0) bulk_g2s(piece0 + (uint32_t)s * piece_bytes, p.b + at, LR_PIECE_BYTES, PTILE(s));
-        return true;
-      });
     }
     if (!ok) __nanosleep(500000);                             // copies in flight land before the block's shared memory goes
     __syncwarp();
@@ -629,6 +645,9 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(ACC_FREE, (tc & 1u) ^ 1u, ctl, 1113));
         if (!ok) break;
         tc_fence_after();
+        // this split's pieces of the block: every S-th
+        const int total = p.list ? __shfl_sync(0xFFFFFFFFu, p.list[(int64_t)(tile / pl.tiles_n) * LR_LIST + 1], 0) : 0;
+        const int end = m + (total > split ? (total - split + S - 1) / S : 0);
         for (int kt = kt0; kt < kt1; ++kt, ++it) {
           const int s = it % pl.stages;
           ok = __all_sync(0xFFFFFFFFu, mbar_wait(FULL(s), (it / pl.stages) & 1u, ctl, 1114));
@@ -641,9 +660,10 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
               elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo + kk * 2, b_lo + (uint32_t)(j * half * 8) + kk * 2, DESC_HI, idesc, kt > kt0 || kk > 0 ? 1u : 0u);
           elect_commit_both(EMPTY(s), both);
         }
-        ok = ok && pieces(tile / pl.tiles_n, m, [&](int m, int, int) {
+        for (; m < end && ok; ++m) {
           const int s = m % pl.pieces;
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(PFULL(s), (m / pl.pieces) & 1u, ctl, 1115))) return false;
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(PFULL(s), (m / pl.pieces) & 1u, ctl, 1115));
+          if (!ok) break;
           tc_fence_after();
           const uint32_t st = piece0 + (uint32_t)s * piece_bytes, a_lo = piece_desc(st), b_lo = piece_desc(st + LR_PIECE_BYTES);
           for (int j = 0; j < pl.mmas; ++j) {
@@ -651,8 +671,7 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
             elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo, b_lo + (T_BYTES >> 4) + (uint32_t)(j * half * 2), PIECE_DESC_HI, idesc, 1u);
           }
           elect_commit_both(PEMPTY(s), both);
-          return true;
-        });
+        }
         if (ok) elect_commit_both(ACC, both);
       }
       elect_commit_pair_local(DRAIN);                         // every MMA has retired before tensor memory is freed
@@ -689,27 +708,47 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
       if (lane == 0) mbar_arrive_cluster(ACC_FREE, even);
     }
   } else {
-    // ================================= tokens' side of the pieces ===================================================
+    // ================================= pieces ==================================================================
     int m = 0;
     bool ok = true;
-    for (int tile = tile0; tile < tile1 && ok; ++tile) {
-      const int block = tile / pl.tiles_n;
-      ok = pieces(block, m, [&](int m, int a, int i) {
-        const int s = m % pl.pieces;
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1117))) return false;
-        const uint32_t dst = piece0 + (uint32_t)s * piece_bytes + LR_PIECE_BYTES;
-        for (int r = (warp - 6) * 32 + lane; r < TB / 2; r += 128) {
-          const int j = r >= half ? 1 : 0;
-          const int64_t token = (int64_t)block * TB + j * n_mma + (int)half_id * half + (r - j * half);
-          write_piece_row<T16>(p, token < p.T && p.indx[token] == a, token, i * LR_PIECE, dst, T_BYTES, r);
+    for (int tile = tile0; tile < tile1 && ok && p.list; ++tile) {
+      const int block = tile / pl.tiles_n, n0 = (tile - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
+      const int32_t* list = p.list + (int64_t)block * LR_LIST;
+      const int n = list[0];
+      int g = 0, my_a = 0, my_first = 0, my_np = 0;           // the block's adapters 32 at a time, one a lane
+      for (int l = 0; l < n && ok; ++l) {
+        if ((l & 31) == 0 && l + lane < n) {
+          my_a = list[2 + l + lane];
+          my_first = p.first[my_a];
+          my_np = p.first[my_a + 1] - my_first;
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (warp == 6 && !__all_sync(0xFFFFFFFFu, mbar_wait(PTILE(s), (m / pl.pieces) & 1u, ctl, 1118))) return false;
-        if (lane == 0) mbar_arrive_cluster(PFULL(s), even);
-        return true;
-      });
+        const int a = __shfl_sync(0xFFFFFFFFu, my_a, l & 31), first = __shfl_sync(0xFFFFFFFFu, my_first, l & 31), np = __shfl_sync(0xFFFFFFFFu, my_np, l & 31);
+        for (int i = 0; i < np && ok; ++i, ++g) {
+          if (g % S != split) continue;
+          const int s = m % pl.pieces;
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(PEMPTY(s), ((m / pl.pieces) & 1u) ^ 1u, ctl, 1112));
+          if (!ok) break;
+          const uint32_t dst = piece0 + (uint32_t)s * piece_bytes;
+          if (warp == 6 && lane == 0) {
+            mbar_expect_tx(PTILE(s), LR_PIECE_BYTES);
+            // (rows of B are padded to 128: the odd CTA of the last tile may have none)
+            bulk_g2s(dst, p.b + ((int64_t)(first + i) * p.NP + (n0 < p.NP ? n0 : 0)) * 32, LR_PIECE_BYTES, PTILE(s));
+          }
+          for (int r = (warp - 6) * 32 + lane; r < TB / 2; r += 128) {
+            const int j = r >= half ? 1 : 0;
+            const int64_t token = (int64_t)block * TB + j * n_mma + (int)half_id * half + (r - j * half);
+            write_piece_row<T16>(p, token < p.T && p.indx[token] == a, token, i * LR_PIECE, dst + LR_PIECE_BYTES, T_BYTES, r);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (warp == 6) ok = __all_sync(0xFFFFFFFFu, mbar_wait(PTILE(s), (m / pl.pieces) & 1u, ctl, 1117));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_cluster(PFULL(s), even);
+          ++m;
+        }
+      }
     }
+    if (!ok) __nanosleep(500000);
   }
   tc_fence_before();
   __syncthreads();
@@ -727,7 +766,7 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
       const int block = tile0 / pl.tiles_n, n0 = (tile0 - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
       const int64_t row0 = (int64_t)block * TB;
       const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0);
-      cluster_sums<T16>(p, sbase, S, 2u, half_id, row0, rows * split / S, rows * (split + 1) / S, n0);
+      cluster_sums<T16, LP_MAX_SPLITS, 4>(p, sbase, S, 2u, half_id, row0, rows * split / S, rows * (split + 1) / S, n0);
     }
     cluster_sync_all();                                       // no CTA leaves while its sums are read
   }
@@ -772,15 +811,13 @@ int lr_map(const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows, 
 struct ShrinkPlan { int nb, places, parts; };
 ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   ShrinkPlan s;
-  s.nb = T <= 128 ? 1 : 8;
-  const int64_t blocks = cdiv64(T, 8 * s.nb);
-  const int64_t most = n_adapters < 8 * s.nb ? n_adapters : 8 * s.nb;             // adapters that a block can hold
-  const int64_t want = s.nb == 1 ? 8 : T <= 1024 ? 16 : 4;      // (a place without an adapter costs a block of threads all the same)
-  s.places = (int)(most < want ? most : want);
-  // shares of k up to as many blocks with something to do as there are SMs, twice as many of the long ones
-  const int64_t enough = moe_sm_count() * (s.nb == 1 ? 1 : 2);
+  s.nb = T <= 1024 ? 1 : 8;
+  const int most = s.nb == 1 ? 8 : 4;                         // (a place without an adapter costs a block of threads all the same)
+  s.places = n_adapters < most ? n_adapters : most;
+  // shares of k while the blocks that have something to do, a quarter of them say, are fewer than the SMs
+  const int64_t blocks = cdiv64(T, 8 * s.nb) * max_pieces * (s.nb == 1 && s.places > 2 ? s.places / 2 : 1);
   int parts = 1;
-  while (parts < 8 && blocks * max_pieces * parts * 2 <= enough && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
+  while (parts < 4 && blocks * parts <= moe_sm_count() && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
   s.parts = parts;
   return s;
 }
@@ -794,7 +831,7 @@ StreamPlan lr_stream_plan(int64_t T, int K, int N) {
   // to six CTAs and 29.7 in clusters of seven (280 CTAs of 296), where some wait for a second round.
   int64_t s = moe_sm_count() * 5 / 3 / tiles;
   if (s > KT / 4) s = KT / 4;
-  pl.splits = (int)(s < 1 ? 1 : s > 6 ? 6 : s);
+  pl.splits = (int)(s < 1 ? 1 : s > LS_MAX_SPLITS ? LS_MAX_SPLITS : s);
   const int st = (104 * 1024 - sums) / stage;
   pl.stages = st > LS_MAX_STAGES ? LS_MAX_STAGES : st;
   pl.smem = pl.stages * stage + sums + 1024;                  // (the product's sums take the ring's place: two stages are enough for them)
@@ -841,7 +878,7 @@ PairPlan lr_pair_plan(int64_t T, int K, int N) {
     int64_t tb = cdiv64(cdiv64(T, nb), 32) * 32;
     if (tb < 64) tb = 64;
     const int64_t blocks = cdiv64(T, tb), tiles = tiles_n * blocks;
-    int64_t s = tb > 416 ? 1 : KT / 4 < 4 ? KT / 4 : 4;       // (a split's sums are tb x 128 fp32 in shared memory)
+    int64_t s = tb > 416 ? 1 : KT / 4 < LP_MAX_SPLITS ? KT / 4 : LP_MAX_SPLITS;       // (a split's sums are tb x 128 fp32 in shared memory)
     while (s > 1 && tiles > lr_pair_clusters((int)s)) --s;
     if (s < 1) s = 1;
     const double rounds = (double)cdiv64(tiles, lr_pair_clusters((int)s));
@@ -854,7 +891,7 @@ PairPlan lr_pair_plan(int64_t T, int K, int N) {
   }
   best.mmas = best.tb > 256 ? 2 : 1;
   const int stage = SUBTILE_BYTES + best.tb * 64, piece = LR_PIECE_BYTES + best.tb * 32, room = 224 * 1024;
-  best.pieces = best.tb > 256 ? 2 : 4;
+  best.pieces = LP_MAX_PIECES;
   best.stages = (room - best.pieces * piece) / stage;
   if (best.stages > LP_MAX_STAGES) best.stages = LP_MAX_STAGES;
   int bytes = best.stages * stage + best.pieces * piece;

@@ -132,10 +132,10 @@ _STATUS_TEXT = {
     1005: "layer of a few tokens: the epilogue waited for a unit's sums", 1006: "layer of a few tokens: a warp waited for a free buffer of sums",
     1101: "projection with adapters: the producer waited for a free stage", 1102: "projection with adapters: the MMA warp waited for a stage",
     1103: "projection with adapters: the epilogue waited for the accumulator",
-    1111: "projection with adapters, pairs: the producer waited for a free stage", 1112: "projection with adapters, pairs: the producer waited for a free piece",
+    1111: "projection with adapters, pairs: the producer waited for a free stage", 1112: "projection with adapters, pairs: a writer waited for a free piece",
     1113: "projection with adapters, pairs: the MMA warp waited for a free accumulator", 1114: "projection with adapters, pairs: the MMA warp waited for a stage",
     1115: "projection with adapters, pairs: the MMA warp waited for a piece", 1116: "projection with adapters, pairs: the epilogue waited for the accumulator",
-    1117: "projection with adapters, pairs: a writer waited for a free piece", 1118: "projection with adapters, pairs: a writer waited for a piece's tile",
+    1117: "projection with adapters, pairs: a writer waited for a piece's tile",
 }
 
 
