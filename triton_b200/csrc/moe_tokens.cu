@@ -28,12 +28,13 @@ namespace {
 constexpr int MT_MAX_TOKENS = 16;
 constexpr int MT_MAX_K = 16;              // picks per token
 constexpr int MT_MAX_EXPERTS = 256;
-constexpr int MT_WARPS = 16;              // consumer warps: 8 shares of k times 2 slabs of 16 weight rows
+constexpr int MT_WARPS = 16;              // consumer warps: two teams of 4 shares of k times 2 slabs of 16 weight rows
 constexpr int MT_CONSUMERS = MT_WARPS * 32;
 constexpr int MT_EPILOGUE = 96;           // threads that take the sums on while the consumers are at the next unit
 constexpr int MT_THREADS = MT_CONSUMERS + MT_EPILOGUE + 32;
 constexpr int MT_UNIT = 32;               // weight rows of a unit
-constexpr int MT_STAGE_KT = 8;            // 128-k tiles of a stage, one per share of k
+constexpr int MT_SHARES = 4;              // of k in a team
+constexpr int MT_STAGE_KT = 8;            // 128-k tiles of a stage, two per share of k
 constexpr int MT_STAGE_VALUES = MT_STAGE_KT * 4 * MT_UNIT * 16;
 constexpr int MT_STAGE_BYTES = MT_STAGE_VALUES + MT_STAGE_KT * MT_UNIT * 4;
 constexpr int MT_RED_LD = 36;             // pitch of a column of sums: the quads of an accumulator fragment go to distinct banks
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 127) & ~(uintptr_t)127);
   __shared__ TokensShared s;
-  __shared__ __align__(16) float s_red[2][8][8 * NBLK * MT_RED_LD];    // [buffer][share of k][column][row]
+  __shared__ __align__(16) float s_red[2][MT_SHARES][8 * NBLK * MT_RED_LD];      // [team][share of k][column][row]
   const uint32_t ring = smem_u32(smem), toks = ring + (uint32_t)(p.stages * MT_STAGE_BYTES);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;     // warp-uniform for the compiler
   auto FULL = [&](int i) { return smem_u32(&s.full[i]); };
@@ -363,10 +364,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(FULL(i), 1);
-      mbar_init(EMPTY(i), MT_WARPS);
+      mbar_init(EMPTY(i), MT_WARPS / 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(SUMS(i), MT_WARPS);
+      mbar_init(SUMS(i), MT_WARPS / 2);
       mbar_init(TAKEN(i), MT_EPILOGUE / 32);
     }
     s.abort = 0;
@@ -417,42 +418,42 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     // ================================= weights =================================================================
     // the warp goes through the loop as a whole and elects a lane at each instruction: a thread by itself took longer to issue a stage's copies
     // than they take from HBM
-    int ri = 0;
-    uint32_t rp = 1, it = 0;
+    // Units go to the two teams in turn, each of which has half of the ring for itself.
+    const int half = p.stages / 2;
+    int ri[2] = {0, 0};
+    uint32_t rp[2] = {1, 1};
     bool ok = true;
-    auto stage = [&](const CUtensorMap* v, const CUtensorMap* sc, uint32_t bytes, int nb, int tile) {
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(ri), rp, ctl, 1001));
+    auto stage = [&](int team, const CUtensorMap* v, const CUtensorMap* sc, uint32_t bytes, int nb, int tile) {
+      const int at = team * half + (team ? ri[1] : ri[0]);
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(EMPTY(at), team ? rp[1] : rp[0], ctl, 1001));
       if (!ok) return;
-      const uint32_t dst = ring + (uint32_t)(ri * MT_STAGE_BYTES);
-      elect_expect_tx(FULL(ri), bytes);
-      elect_tile_2d(dst, v, (nb & 3) * 128, tile * 4, FULL(ri));
-      elect_tile_2d(dst + MT_STAGE_VALUES, sc, (nb & 3) * 32, tile, FULL(ri));
-      if (++ri == p.stages) { ri = 0; rp ^= 1u; }
-      ++it;
+      const uint32_t dst = ring + (uint32_t)(at * MT_STAGE_BYTES);
+      elect_expect_tx(FULL(at), bytes);
+      elect_tile_2d(dst, v, (nb & 3) * 128, tile * 4, FULL(at));
+      elect_tile_2d(dst + MT_STAGE_VALUES, sc, (nb & 3) * 32, tile, FULL(at));
+      if (team) { if (++ri[1] == half) { ri[1] = 0; rp[1] ^= 1u; } }
+      else { if (++ri[0] == half) { ri[0] = 0; rp[0] ^= 1u; } }
     };
+    int m = 0;
     // units [from, from + units) of a product, their stages from js0 in the first to js1 in the last
     auto product = [&](const CUtensorMap* v, const CUtensorMap* sc, const CUtensorMap* vt, const CUtensorMap* st, int NB, int NT, int KT, int KS, int from,
                        int units, int js0, int js1) {
       const uint32_t whole = MT_STAGE_KT * MT_UNIT * 68, tail = (uint32_t)((KT - (KS - 1) * MT_STAGE_KT) * MT_UNIT * 68);
       int place = from / NB, nb = from - place * NB;
 #pragma unroll 1
-      for (int m = 0; m < units && ok; ++m) {
-        const int tile = (s.act[place] * NT + (nb >> 2)) * KT, end = m + 1 == units ? js1 : KS;
+      for (int i = 0; i < units && ok; ++i, ++m) {
+        const int tile = (s.act[place] * NT + (nb >> 2)) * KT, end = i + 1 == units ? js1 : KS;
 #pragma unroll 1
-        for (int js = m == 0 ? js0 : 0; js < end && ok; ++js) {
-          if (js < KS - 1) stage(v, sc, whole, nb, tile + js * MT_STAGE_KT);
-          else stage(vt, st, tail, nb, tile + js * MT_STAGE_KT);
+        for (int js = i == 0 ? js0 : 0; js < end && ok; ++js) {
+          if (js < KS - 1) stage(m & 1, v, sc, whole, nb, tile + js * MT_STAGE_KT);
+          else stage(m & 1, vt, st, tail, nb, tile + js * MT_STAGE_KT);
         }
         if (++nb == NB) { nb = 0; ++place; }
       }
     };
     product(&maps.v1, &maps.s1, &maps.v1t, &maps.s1t, NB1, NT1, KT1, KS1, u_begin, n1, 0, KS1);
     product(&maps.v2, &maps.s2, &maps.v2t, &maps.s2t, NB2, NT2, KT2, KS2, first2, n2, s_begin - first2 * KS2, s_end - (first2 + n2 - 1) * KS2);
-    if (!ok && lane == 0) {                                   // copies in flight land before the block's shared memory goes
-      const uint32_t lo = it > (uint32_t)p.stages ? it - p.stages : 0;
-      for (uint32_t j = lo; j < it; ++j)
-        for (uint32_t t = 0; t < (1u << 16) && !mbar_test(FULL(j % p.stages), (j / p.stages) & 1u); ++t) __nanosleep(64);
-    }
+    if (!ok) __nanosleep(500000);                             // copies in flight land before the block's shared memory goes
     return;
   }
 
@@ -493,8 +494,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         const int t = s.who[e][live ? r : 0], entry = t * p.k + s.slot[e][t];
         float g = 0.0f, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const float2 v = *reinterpret_cast<const float2*>(&s_red[m & 1][w][t * MT_RED_LD + 2 * i]);
+        for (int w = 0; w < MT_SHARES; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(&s_red[m & 1][w][(live ? r : 0) * MT_RED_LD + 2 * i]);
           g += v.x;
           l += v.y;
         }
@@ -541,10 +542,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
       for (int r = tid >> 5; r < n; r += MT_EPILOGUE / 32) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) v += s_red[m & 1][w][r * MT_RED_LD + lane_row];
+        for (int w = 0; w < MT_SHARES; ++w) v += s_red[m & 1][w][r * MT_RED_LD + lane_row];
         if (two_terms(n, NBLK)) {
 #pragma unroll
-          for (int w = 0; w < 8; ++w) v += s_red[m & 1][w][(n + r) * MT_RED_LD + lane_row];
+          for (int w = 0; w < MT_SHARES; ++w) v += s_red[m & 1][w][(n + r) * MT_RED_LD + lane_row];
         }
         __stcg(p.part + ((int64_t)(u + c) * p.T + r) * MT_UNIT + lane_row, settle(v, p.s2, e, NT2, KT2, (u % NB2) * MT_UNIT + lane_row) * s.undo2[changes & 3][r]);
       }
@@ -561,53 +562,62 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   }
 
   // ================================= consumers =================================================================
-  const int wk = warp & 7, slab = warp >> 3, qrow = lane >> 2, c4 = lane & 3, tid = threadIdx.x;
+  const int wk = warp & 3, slab = (warp >> 2) & 1, team = warp >> 3, half = p.stages / 2, qrow = lane >> 2, c4 = lane & 3, tid = threadIdx.x;
   // (where a wait runs out, this and the following ones return, the rest is gone through and its results are void)
-  int ri = 0;                           // place in the ring
+  int ri = 0;                           // place in the team's half of the ring
   uint32_t rp = 0;
   float acc[NBLK][4];
-  // This warp's tile of a stage, 16 rows x 128 k, times the columns of NB blocks from `xt` on.  Every load goes ahead of the arithmetic: what bounds
-  // the loop is the number of instructions and the way of one warp through a stage.
-  const uint32_t my_w = ring + (uint32_t)(wk * 2048 + (slab * 16 + qrow) * 16 + c4 * 4), my_s = ring + (uint32_t)(MT_STAGE_VALUES + wk * 128 + (slab * 16 + qrow) * 4);
-  const uint32_t my_x = toks + (uint32_t)(wk * 4 * NBLK * 512 + qrow * 64 + c4 * 16);
-  auto multiply = [&](auto nb_tag, bool live, uint32_t xt) {
+  // This warp's tiles of a stage, 16 rows x 128 k each, times NB blocks of columns, k from `xt` on; `left`: k tiles from the stage on.  Every load of a
+  // tile goes ahead of its arithmetic: what bounds the loop is the number of instructions and the way of one warp through a stage.
+  const uint32_t my_ring = ring + (uint32_t)(team * half * MT_STAGE_BYTES);
+  const uint32_t my_w = my_ring + (uint32_t)(wk * 2048 + (slab * 16 + qrow) * 16 + c4 * 4), my_s = my_ring + (uint32_t)(MT_STAGE_VALUES + wk * 128 + (slab * 16 + qrow) * 4);
+  const uint32_t my_x = toks + (uint32_t)(wk * 4 * NBLK * 512 + c4 * 16);
+  uint32_t col[NBLK];                   // where the lane's columns are
+  auto multiply = [&](auto nb_tag, int left, uint32_t xt) {
     constexpr int NB = decltype(nb_tag)::value;
-    mbar_wait_short(FULL(ri), rp, ctl, 1002);
-    if (live) {
-      const uint32_t wt = my_w + (uint32_t)(ri * MT_STAGE_BYTES), sc = my_s + (uint32_t)(ri * MT_STAGE_BYTES);
-      const uint32_t sl = lds32(sc), sh = lds32(sc + 32);
-      uint32_t wl[4], wh[4];
-      uint4 xb[4][NB];
+    const int at = team * half + ri;
+    mbar_wait_short(FULL(at), rp, ctl, 1002);
+    uint32_t wt = my_w + (uint32_t)(ri * MT_STAGE_BYTES), sc = my_s + (uint32_t)(ri * MT_STAGE_BYTES);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        wl[g] = lds32(wt + g * 512);
-        wh[g] = lds32(wt + g * 512 + 128);
+    for (int h = 0; h < MT_STAGE_KT / MT_SHARES; ++h) {
+      if (wk + h * MT_SHARES < left) {
+        const uint32_t sl = lds32(sc), sh = lds32(sc + 32);
+        uint32_t wl[4], wh[4];
+        uint4 xb[4][NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) xb[g][b] = lds128(xt + (uint32_t)((g * NBLK + b) * 512));
-      }
-      float fl[4], fh[4];
-      e8m0_word(sl, fl);
-      e8m0_word(sh, fh);
+        for (int g = 0; g < 4; ++g) {
+          wl[g] = lds32(wt + g * 512);
+          wh[g] = lds32(wt + g * 512 + 128);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t lo[4], hi[4];
-        e2m1_word(wl[g], lo);
-        e2m1_word(wh[g], hi);
+          for (int b = 0; b < NB; ++b) xb[g][b] = lds128(xt + col[b] + (uint32_t)(g * NBLK * 512));
+        }
+        float fl[4], fh[4];
+        e8m0_word(sl, fl);
+        e8m0_word(sh, fh);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          float dd[4];
-          mma_f16_zero(dd, lo[0], hi[0], lo[1], hi[1], xb[g][b].x, xb[g][b].y);
-          mma_f16(dd, lo[2], hi[2], lo[3], hi[3], xb[g][b].z, xb[g][b].w);
-          acc[b][0] = fmaf(fl[g], dd[0], acc[b][0]);
-          acc[b][1] = fmaf(fl[g], dd[1], acc[b][1]);
-          acc[b][2] = fmaf(fh[g], dd[2], acc[b][2]);
-          acc[b][3] = fmaf(fh[g], dd[3], acc[b][3]);
+        for (int g = 0; g < 4; ++g) {
+          uint32_t lo[4], hi[4];
+          e2m1_word(wl[g], lo);
+          e2m1_word(wh[g], hi);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            float dd[4];
+            mma_f16_zero(dd, lo[0], hi[0], lo[1], hi[1], xb[g][b].x, xb[g][b].y);
+            mma_f16(dd, lo[2], hi[2], lo[3], hi[3], xb[g][b].z, xb[g][b].w);
+            acc[b][0] = fmaf(fl[g], dd[0], acc[b][0]);
+            acc[b][1] = fmaf(fl[g], dd[1], acc[b][1]);
+            acc[b][2] = fmaf(fh[g], dd[2], acc[b][2]);
+            acc[b][3] = fmaf(fh[g], dd[3], acc[b][3]);
+          }
         }
       }
+      wt += MT_SHARES * 2048;
+      sc += MT_SHARES * 128;
+      xt += MT_SHARES * 4 * NBLK * 512;
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(EMPTY(ri));
-    if (++ri == p.stages) { ri = 0; rp ^= 1u; }
+    if (lane == 0) mbar_arrive(EMPTY(at));
+    if (++ri == half) { ri = 0; rp ^= 1u; }
   };
 
   if (NBLK == 2) {
@@ -616,7 +626,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   }
   // ---- all units, fc1's and fc2's ----
   int have = -1, changes = -1;          // expert whose rows of fc2 are staged
-  int first = 0, n_blocks = 1;          // blocks of columns that the expert's tokens are in
+  int n_blocks = 1;                     // of the expert's tokens as columns
   int place = u_begin / NB1, rest = u_begin - place * NB1;   // the unit's expert in the list of active ones, its place among the expert's units
 #pragma unroll 1
   for (int m = 0; m < n1 + n2; ++m, ++rest) {
@@ -627,8 +637,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     const int js0 = m == n1 ? s_begin - first2 * KS2 : 0, js1 = one ? KS1 : m + 1 == n1 + n2 ? s_end - (first2 + n2 - 1) * KS2 : KS2;
     const uint32_t mask = s.tokens[e];
     if (one) {
-      first = mask & 0xFFu ? 0 : 1;
-      n_blocks = NBLK == 2 && !first && mask >> 8 ? 2 : 1;
+      n_blocks = __popc(mask) > 8 ? 2 : 1;                    // fc1's columns are the expert's tokens among those of the batch
+#pragma unroll
+      for (int b = 0; b < NBLK; ++b) {
+        const int t = s.who[e][b * 8 + qrow] & (MT_MAX_TOKENS - 1);      // (any column stands in for one without a token)
+        col[b] = (uint32_t)((t >> 3) * 512 + (t & 7) * 64) & (uint32_t)(NBLK * 512 - 1);
+      }
     } else if (e != have) {
       if (tid == 0) wait_count(p.done1 + e, NB1, ctl, 1003);
       bar_sync(1, MT_CONSUMERS);                              // fc1's rows are there, and the staged ones have been read
@@ -637,30 +651,31 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
       stage_h(p, s, NBLK, toks, e, n, KT2, changes & 3, warp);
       bar_sync(1, MT_CONSUMERS);
       have = e;
-      first = 0;
       n_blocks = (two_terms(n, NBLK) ? 2 * n : n) > 8 ? 2 : 1;
+#pragma unroll
+      for (int b = 0; b < NBLK; ++b) col[b] = (uint32_t)(b * 512 + qrow * 64);
     }
+    if ((m & 1) != team) continue;                            // the other team's
 #pragma unroll
     for (int b = 0; b < NBLK; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[b][j] = 0.0f;
     uint32_t xt = my_x + (uint32_t)(js0 * MT_STAGE_KT * 4 * NBLK * 512);
     if (NBLK == 1 || n_blocks == 1) {
-      xt += (uint32_t)(first * 512);
 #pragma unroll 1
       for (int js = js0; js < js1; ++js, xt += MT_STAGE_KT * 4 * NBLK * 512)
-        multiply(std::integral_constant<int, 1>(), js * MT_STAGE_KT + wk < KT, xt);
+        multiply(std::integral_constant<int, 1>(), KT - js * MT_STAGE_KT, xt);
     } else {
 #pragma unroll 1
       for (int js = js0; js < js1; ++js, xt += MT_STAGE_KT * 4 * NBLK * 512)
-        multiply(std::integral_constant<int, NBLK>(), js * MT_STAGE_KT + wk < KT, xt);
+        multiply(std::integral_constant<int, NBLK>(), KT - js * MT_STAGE_KT, xt);
     }
-    // the warp's share of the unit's sums goes to the epilogue; two buffers
+    // the warp's share of the unit's sums goes to the epilogue; a buffer per team
     if (m >= 2) mbar_wait_short(TAKEN(m & 1), ((m >> 1) & 1u) ^ 1u, ctl, 1006);
 #pragma unroll
     for (int b = 0; b < NBLK; ++b)
       if (b < n_blocks) {
-        float* at = &s_red[m & 1][wk][((first + b) * 8 + c4 * 2) * MT_RED_LD + slab * 16 + qrow];
+        float* at = &s_red[m & 1][wk][(b * 8 + c4 * 2) * MT_RED_LD + slab * 16 + qrow];
         at[0] = acc[b][0];
         at[MT_RED_LD] = acc[b][1];
         at[8] = acc[b][2];
@@ -802,7 +817,7 @@ template <int NBLK> int mt_launch(TokensParams& p, const TokensMaps& maps, cudaS
   const int width = p.d > p.ff ? p.d : p.ff;
   p.tok_bytes = (int)cdiv64(width, 128) * 4 * 512 * NBLK;
   const int left = MT_SMEM - mt_static_smem<NBLK>() - 128 - p.tok_bytes;
-  p.stages = left / MT_STAGE_BYTES < MT_MAX_STAGES ? left / MT_STAGE_BYTES : MT_MAX_STAGES;
+  p.stages = (left / MT_STAGE_BYTES < MT_MAX_STAGES ? left / MT_STAGE_BYTES : MT_MAX_STAGES) & ~1;      // half for each team
   if (p.stages < 2) {
     moe_set_error("moe_layer_tokens: no shared memory left for weights (d = %d, ff = %d)", p.d, p.ff);
     return MOE_ERR_UNSUPPORTED;
