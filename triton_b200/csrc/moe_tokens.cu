@@ -139,6 +139,10 @@ __device__ __forceinline__ void e2m1_word(uint32_t w, uint32_t (&h)[4]) {
       "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\tcvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
+// four matrices of 8 rows x 16 bytes at the lanes' addresses: a lane has word lane % 4 of row lane / 4 of each
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr));
+}
 __device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
@@ -570,7 +574,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   // This warp's tiles of a stage, 16 rows x 128 k each, times NB blocks of columns, k from `xt` on; `left`: k tiles from the stage on.  Every load of a
   // tile goes ahead of its arithmetic: what bounds the loop is the number of instructions and the way of one warp through a stage.
   const uint32_t my_ring = ring + (uint32_t)(team * half * MT_STAGE_BYTES);
-  const uint32_t my_w = my_ring + (uint32_t)(wk * 2048 + (slab * 16 + qrow) * 16 + c4 * 4), my_s = my_ring + (uint32_t)(MT_STAGE_VALUES + wk * 128 + (slab * 16 + qrow) * 4);
+  // (the eight rows of a matrix that the lane addresses: rows 0-7 and 8-15 of two groups of 32 k)
+  const uint32_t my_w = my_ring + (uint32_t)(wk * 2048 + (lane >> 4) * 512 + (slab * 16 + (lane & 15)) * 16), my_s = my_ring + (uint32_t)(MT_STAGE_VALUES + wk * 128 + (slab * 16 + qrow) * 4);
   const uint32_t my_x = toks + (uint32_t)(wk * 4 * NBLK * 512 + c4 * 16);
   uint32_t col[NBLK];                   // where the lane's columns are
   auto multiply = [&](auto nb_tag, int left, uint32_t xt) {
@@ -584,10 +589,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         const uint32_t sl = lds32(sc), sh = lds32(sc + 32);
         uint32_t wl[4], wh[4];
         uint4 xb[4][NB];
+        ldmatrix_x4(wt, wl[0], wh[0], wl[1], wh[1]);
+        ldmatrix_x4(wt + 1024, wl[2], wh[2], wl[3], wh[3]);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          wl[g] = lds32(wt + g * 512);
-          wh[g] = lds32(wt + g * 512 + 128);
 #pragma unroll
           for (int b = 0; b < NB; ++b) xb[g][b] = lds128(xt + col[b] + (uint32_t)(g * NBLK * 512));
         }
