@@ -93,3 +93,192 @@ def test_shapes(T, K, N, ranks, kind):
 @pytest.mark.parametrize("T", [3, 500])
 def test_high_rank(T):
     run_case(T, 256, 256, [1024, 200], kind="random", seed=5)
+
+
+@gpu
+@pytest.mark.parametrize("T,K,N,ranks", [(5000, 64, 5120, [16, 40]), (1500, 8, 9000, [16] * 9), (8200, 128, 300, [1])])
+def test_more_tiles_than_pairs(T, K, N, ranks):
+    run_case(T, K, N, ranks, kind="runs", seed=7)
+
+
+@gpu
+@pytest.mark.parametrize("T", [20, 200])
+def test_many_adapters(T):
+    run_case(T, 64, 200, [1 + i % 20 for i in range(300)], seed=9)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [1, 40, 700])
+def test_without_adapters(T, dtype):
+    x, w, b, *_ = make(T, 200, 333, [], dtype, 4)
+    w = tb.prepare_projection_weight(w)
+    check(tb.matmul_lora(x, w, b, None, None), *reference(x, w, b, [], [], [], torch.full((T,), -1, device="cuda")))
+
+
+@gpu
+@pytest.mark.parametrize("T", [10, 300])
+def test_a_request_that_is_not_finite_stays_by_itself(T):
+    x, w, b, la, lb, scale = make(T, 256, 200, [16, 24, 8], torch.bfloat16, 5)
+    indx = indices(T, 3, "random", 5)
+    w, adapters = tb.prepare_projection_weight(w), tb.prepare_lora_adapters(la, lb, scale)
+    want = tb.matmul_lora(x, w, b, adapters, indx)
+    y = x.clone()
+    y[3, 5] = float("nan")
+    y[4, 6] = float("inf")
+    got = tb.matmul_lora(y, w, b, adapters, indx)
+    assert torch.equal(got[:3], want[:3]) and torch.equal(got[5:], want[5:]) and not torch.isfinite(got[3:5]).any()
+    broken = [la[0].clone(), *la[1:]]
+    broken[0][2, 2] = float("inf")                             # an adapter that has gone wrong
+    got = tb.matmul_lora(x, w, b, tb.prepare_lora_adapters(broken, lb, scale), indx)
+    assert torch.equal(got[indx != 0], want[indx != 0]) and not torch.isfinite(got[indx == 0]).any()
+
+
+@gpu
+@pytest.mark.parametrize("T", [10, 300])
+def test_layouts_of_the_inputs(T):
+    x, w, b, la, lb, scale = make(T, 256, 200, [16, 24, 8], torch.bfloat16, 6)
+    indx = indices(T, 3, "random", 6)
+    pw, adapters = tb.prepare_projection_weight(w), tb.prepare_lora_adapters(la, lb, scale)
+    want = tb.matmul_lora(x, pw, b, adapters, indx)
+    wide = torch.full((T, 600), float("nan"), device="cuda", dtype=x.dtype)
+    wide[:, 129:385] = x
+    assert torch.equal(tb.matmul_lora(wide[:, 129:385], pw, b, adapters, indx), want)
+    assert torch.equal(tb.matmul_lora(x.t().contiguous().t(), pw, b, adapters, indx), want)
+    assert torch.equal(tb.matmul_lora(x, w, b, adapters, indx), want)                                   # a weight not prepared
+    assert torch.equal(tb.matmul_lora(x, pw, b.float(), adapters, indx), want)
+    both = torch.stack((indx, indx), 1)[:, 0]
+    assert torch.equal(tb.matmul_lora(x, pw, b, adapters, both), want)                                  # a strided index
+    far = indx.long().masked_fill(indx == -1, 1 << 40)
+    assert torch.equal(tb.matmul_lora(x, pw, b, adapters, far), want)                                   # past the last adapter is none
+    assert torch.equal(tb.matmul_lora(x, pw, b, adapters, indx.masked_fill(indx == -1, 3)), want)
+    assert torch.equal(tb.matmul_lora(x[:0], pw, b, adapters, indx[:0]), want[:0])
+
+
+@gpu
+@pytest.mark.parametrize("T", [10, 300])
+def test_captured_replayed_and_side_by_side(T):
+    cases = []
+    for seed in (1, 2):
+        x, w, b, la, lb, scale = make(T, 512, 640, [16, 8, 32], torch.bfloat16, seed)
+        cases.append((x, tb.prepare_projection_weight(w), b, tb.prepare_lora_adapters(la, lb, scale), indices(T, 3, "random", seed)))
+    want = [tb.matmul_lora(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams, graphs, out = [torch.cuda.Stream() for _ in cases], [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.append(tb.matmul_lora(*c))
+        graphs.append(g)
+    eager = [[], []]
+    for _ in range(10):
+        for c, s, g, e in zip(cases, streams, graphs, eager):
+            with torch.cuda.stream(s):
+                g.replay()
+                e.append(tb.matmul_lora(*c))
+    torch.cuda.synchronize()
+    tb.matmul_check_status()
+    for w_, y, e in zip(want, out, eager):
+        assert torch.equal(w_, y) and all(torch.equal(w_, q) for q in e)
+    for c in cases:                                            # new tokens and new adapters for the captured call
+        c[0].normal_()
+        c[4].copy_(torch.flip(c[4], (0,)))
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for c, y in zip(cases, out):
+        assert torch.equal(y, tb.matmul_lora(*c))
+
+
+@gpu
+def test_a_decode_step_projection_and_expert_layer():
+    """A step of seven requests: attention's output projection with each request's adapter, the residual, the expert layer; eager and in one graph"""
+    from test_moe_tokens_gpu import make_layer, router
+    from test_moe_tokens_gpu import reference as layer_reference
+    T, d, E, k = 7, 256, 16, 4
+    x, w, b, la, lb, scale = make(T, 320, d, [8, 16], torch.bfloat16, 21)
+    residual = torch.randn(T, d, device="cuda").bfloat16()
+    indx = torch.tensor([0, 1, -1, 1, 0, 1, -1], device="cuda", dtype=torch.int32)
+    pw, adapters = tb.prepare_projection_weight(w), tb.prepare_lora_adapters(la, lb, scale)
+    lw, full1, full2 = make_layer(E, d, 192, 21)
+    wg, bg = router(d, E, 21)
+
+    def step():
+        h = tb.matmul_lora(x, pw, b, adapters, indx) + residual
+        return h, h + tb.moe_layer_tokens(h, wg, bg, lw, k)
+
+    h, y = step()
+    ref, bound = reference(x, w, b, la, lb, scale, indx)
+    check(h, ref + residual.double(), bound + 2.0 ** -8 * (ref + residual.double()).abs() + 2.0 ** -8 * bound)
+    ref, bound = layer_reference(h, wg, bg, lw, full1, full2, k)
+    total = h.double() + ref
+    check(y, total, bound + 2.0 ** -8 * (total.abs() + bound))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        _, again = step()
+    g.replay()
+    torch.cuda.synchronize()
+    tb.matmul_check_status()
+    assert torch.equal(again, y)
+
+
+@gpu
+def test_refusals():
+    x, w, b, la, lb, scale = make(4, 64, 96, [16], torch.bfloat16, 0)
+    adapters, indx = tb.prepare_lora_adapters(la, lb, scale), torch.zeros(4, dtype=torch.int32, device="cuda")
+    good = {"x": x, "w": w, "bias": b, "adapters": adapters, "indx": indx}
+    other = tb.prepare_lora_adapters([la[0][:32]], lb, scale)
+    bad = [dict(x=x.float()), dict(x=x[0]), dict(x=x[:, :32]), dict(w=w.half()), dict(w=w[None]), dict(bias=b[:5]), dict(bias=b.double()), dict(indx=None),
+           dict(adapters=None), dict(indx=indx[:2]), dict(indx=indx.to(torch.int16)), dict(adapters=other), dict(x=x.half(), w=w.half()), dict(indx=indx.cpu()),
+           dict(w=w.cpu()), dict(bias=b.cpu())]
+    for change in bad:
+        with pytest.raises(ValueError):
+            tb.matmul_lora(**{**good, **change})
+
+
+def test_prepared_adapters():
+    """Layout and refusals of the preparation, which runs anywhere"""
+    x, w, b, la, lb, scale = make(1, 20, 130, [3, 17], torch.bfloat16, 0, device="cpu")
+    p = tb.prepare_lora_adapters(la, lb, scale)
+    assert p.first.tolist() == [0, 1, 3] and p.max_pieces == 2 and p.n_adapters == 2 and p.ranks == (3, 17)
+    assert tuple(p.a.shape) == (48, 24) and tuple(p.b.shape) == (3, 32, 2, 8, 8)
+    rows = p.b.permute(0, 2, 4, 1, 3).reshape(3, 16, 256)      # [piece, rank, output]
+    for i, (r, f) in enumerate(((3, 0), (17, 1))):
+        got = rows[f:f + -(-r // 16)].reshape(-1, 256)
+        assert torch.equal(got[:r, :130], lb[i]) and got[r:].count_nonzero() == 0 and got[:, 130:].count_nonzero() == 0
+        a = p.a[16 * f:16 * f + r]
+        assert torch.equal(a[:, :20], la[i].t()) and a[:, 20:].count_nonzero() == 0
+    nan = lb[0].clone()
+    nan[0, 0] = float("inf")
+    for args in (([], [], []), (la, lb[:1], scale), (la, [nan, lb[1]], scale), ([la[0].float(), la[1]], lb, scale), ([a.float() for a in la], [q.float() for q in lb], scale),
+                 ([la[0][:10], la[1]], lb, scale), (la, [lb[0][:, :5], lb[1]], scale), ([la[0][:, :0], la[1]], [lb[0][:0], lb[1]], scale),
+                 ([torch.zeros(20, 1025).bfloat16()], [torch.zeros(1025, 130).bfloat16()], [1.0])):
+        with pytest.raises(ValueError):
+            tb.prepare_lora_adapters(*args)
+
+
+def test_prepared_weight():
+    w = torch.randn(20, 6).bfloat16()
+    p = tb.prepare_projection_weight(w)
+    assert torch.equal(p, w) and p.stride(0) == 1 and p.stride(1) == 24
+    assert tb.prepare_projection_weight(p) is p
+    for bad in (w.float(), w[None]):
+        with pytest.raises(ValueError):
+            tb.prepare_projection_weight(bad)
+
+
+def test_refuses_cpu_tensors_and_wrong_types():
+    for x in (torch.zeros(1, 32, dtype=torch.bfloat16), torch.zeros(1, 32), torch.zeros(32, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            tb.matmul_lora(x, None, None, None, None)
+
+
+def test_refusals_of_the_c_entry_point():
+    import ctypes
+    from triton_b200 import _lib
+    lib = _lib.load()
+    assert lib.moe_lora_matmul(None, None) == 1 and b"NULL" in lib.moe_last_error()
+    assert lib.moe_lora_matmul_workspace_bytes(None) == 0
+    blank = (ctypes.c_uint8 * 512)()
+    assert lib.moe_lora_matmul(ctypes.addressof(blank), None) == 1 and b"positive" in lib.moe_last_error()

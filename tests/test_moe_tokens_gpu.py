@@ -136,3 +136,187 @@ def test_without_router_bias_and_with_other_activation():
     run_case(3, 8, 2, 256, 256, bias=False)
     run_case(3, 8, 2, 256, 256, limit=None, alpha=1.0, seed=5)
     run_case(3, 8, 2, 256, 256, bias_dtype=torch.float32, limit=0.5, seed=6)
+
+
+def small(T=5, E=8, k=3, d=128, ff=96, seed=11, dtype=torch.bfloat16):
+    lw, full1, full2 = make_layer(E, d, ff, seed)
+    wg, bg = router(d, E, seed)
+    x = torch.randn(T, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+    return x, wg, bg, lw, k, full1, full2
+
+
+@gpu
+def test_equal_logits_go_to_the_lower_expert():
+    x, wg, bg, lw, k, full1, full2 = small()
+    wg = tb.prepare_router_weight(torch.zeros_like(wg).contiguous())
+    bg = torch.tensor([0.0, 1.0, 1.0, 1.0, 1.0, 0.5, 0.0, -1.0], device="cuda")            # four equal logits for three places
+    check(tb.moe_layer_tokens(x, wg, bg, lw, k), *reference(x, wg, bg, lw, full1, full2, k))
+    only = torch.full((8,), float("-inf"), device="cuda")
+    only[6] = 0.25                                             # all but one expert closed: the others have no weight
+    ref, bound = reference(x, wg, torch.where(only.isinf(), -100.0, only), lw, full1, full2, 1)
+    check(tb.moe_layer_tokens(x, wg, only, lw, k), ref, bound)
+    lowest = torch.where(only.isinf(), torch.finfo(torch.float32).min, only)
+    check(tb.moe_layer_tokens(x, wg, lowest, lw, k), ref, bound)
+
+
+@gpu
+@pytest.mark.parametrize("T", [4, 12])
+def test_a_row_that_is_not_finite_stays_by_itself(T):
+    x, wg, bg, lw, k, full1, full2 = small(T)
+    want = tb.moe_layer_tokens(x, wg, bg, lw, k)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        y = x.clone()
+        y[1, 7] = bad
+        got = tb.moe_layer_tokens(y, wg, bg, lw, k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+        assert not torch.isfinite(got[1]).all()
+    y = x.clone()
+    y[1] = 0
+    y[2] *= 2.0 ** -100
+    y[3] *= 2.0 ** 60
+    assert torch.isfinite(tb.moe_layer_tokens(y, wg, bg, lw, k)).all()
+    ref, bound = reference(y[1:3], wg, bg, lw, full1, full2, k)
+    check(tb.moe_layer_tokens(y, wg, bg, lw, k)[1:3], ref, bound)
+
+
+@gpu
+def test_scale_bytes_at_their_ends():
+    E, d, ff = 2, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def laid_out(q, s):
+        return (tb.convert_layout(tb.wrap_torch_tensor(q.transpose(1, 2), dtype=tb.FP4), make_default_matmul_mxfp4_w_layout(mx_axis=-2)),
+                tb.convert_layout(tb.wrap_torch_tensor(s.transpose(1, 2)), make_default_matmul_mxfp4_w_scale_layout(mx_axis=-2)))
+
+    def layer(s1, s2):
+        return MoeLayerWeights(*laid_out(q1, s1), torch.zeros(E, 2 * ff, device="cuda").bfloat16(), *laid_out(q2, s2), torch.zeros(E, d, device="cuda").bfloat16())
+
+    q1 = torch.randint(0, 256, (E, 2 * ff, d // 2), device="cuda", generator=g, dtype=torch.uint8) | 0x11          # no code is zero
+    q2 = torch.randint(0, 256, (E, d, ff // 2), device="cuda", generator=g, dtype=torch.uint8) | 0x11
+    s1 = torch.full((E, 2 * ff, d // 32), 122, device="cuda", dtype=torch.uint8)
+    s2 = torch.full((E, d, ff // 32), 122, device="cuda", dtype=torch.uint8)
+    x = torch.randn(3, d, device="cuda", generator=g).bfloat16()
+    wg, bg = router(d, E, 0)
+    want = tb.moe_layer_tokens(x, wg, bg, layer(s1, s2), 2)
+    assert torch.isfinite(want).all()
+    nan2 = s2.clone()
+    nan2[:, 5, 1] = 255                                        # the dequantiser makes such a group NaN: one output of every expert
+    got = tb.moe_layer_tokens(x, wg, bg, layer(s1, nan2), 2)
+    assert got[:, 5].isnan().all() and torch.equal(torch.cat((got[:, :5], got[:, 6:]), 1), torch.cat((want[:, :5], want[:, 6:]), 1))
+    nan1 = s1.clone()
+    nan1[:, 9, 0] = 255                                        # a hidden value, and with it every output
+    assert tb.moe_layer_tokens(x, wg, bg, layer(nan1, s2), 2).isnan().all()
+    zero2 = s2.clone()
+    zero2[:, 5, :] = 0                                         # byte 0 is the factor 0
+    assert (tb.moe_layer_tokens(x, wg, bg, layer(s1, zero2), 2)[:, 5] == 0).all()
+
+
+@gpu
+def test_layouts_of_the_inputs():
+    x, wg, bg, lw, k, _, _ = small()
+    want = tb.moe_layer_tokens(x, wg, bg, lw, k)
+    wide = torch.zeros(5, 3 * 128 + 1, device="cuda", dtype=x.dtype)
+    wide[:, 129:257] = x
+    assert torch.equal(tb.moe_layer_tokens(wide[:, 129:257], wg, bg, lw, k), want)                      # rows that start anywhere
+    assert torch.equal(tb.moe_layer_tokens(x.t().contiguous().t(), wg, bg, lw, k), want)                # columns together
+    assert torch.equal(tb.moe_layer_tokens(x, wg.contiguous(), bg, lw, k), want)                        # a router weight not prepared
+    shifted = torch.zeros(8 * 128 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(8, 128)
+    shifted.copy_(wg.t())
+    assert torch.equal(tb.moe_layer_tokens(x, shifted.t(), bg, lw, k), want)
+    assert torch.equal(tb.moe_layer_tokens(x[:0], wg, bg, lw, k), want[:0])
+    for t in range(5):                                         # a token's result does not depend on the others but for the rounding of operands
+        one = tb.moe_layer_tokens(x[t:t + 1], wg, bg, lw, k)
+        assert (one - want[t]).float().norm() <= 2.0 ** -8 * want[t].float().norm()
+
+
+@gpu
+def test_the_same_bits_every_time_and_side_by_side():
+    cases = [small(16, 32, 4, 512, 256, seed=1), small(3, 8, 2, 256, 512, seed=2)]
+    want = [tb.moe_layer_tokens(*c[:5]) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(30):
+        for c, s, g in zip(cases, streams, got):
+            with torch.cuda.stream(s):
+                g.append(tb.moe_layer_tokens(*c[:5]))
+    torch.cuda.synchronize()
+    tb.matmul_check_status()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, y) for y in g)
+
+
+@gpu
+def test_two_captured_calls_replayed_side_by_side():
+    cases = [small(4, 8, 2, 256, 128, seed=3), small(4, 8, 2, 256, 128, seed=4)]
+    for c in cases:
+        tb.moe_layer_tokens(*c[:5])
+    torch.cuda.synchronize()
+    graphs, out = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.append(tb.moe_layer_tokens(*c[:5]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in cases]
+    for round_ in range(4):
+        fresh = [torch.randn(4, 256, device="cuda", generator=torch.Generator(device="cuda").manual_seed(100 + round_ + i)).bfloat16() for i in range(2)]
+        for c, f in zip(cases, fresh):
+            c[0].copy_(f)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        tb.matmul_check_status()
+        for c, y in zip(cases, out):
+            assert torch.equal(y, tb.moe_layer_tokens(*c[:5]))
+        torch.cuda.synchronize()
+
+
+@gpu
+def test_agrees_with_the_layer_made_of_operators():
+    x, wg, bg, lw, k, full1, full2 = small(9, 16, 4, 512, 320, seed=8)
+    from triton_b200.moe import moe_layer_forward
+    logits = (x.double() @ wg.double() + bg.double()).float()
+    other = moe_layer_forward(x, logits, lw, k).float()
+    mine = tb.moe_layer_tokens(x, wg, bg, lw, k).float()
+    # the operators round the hidden rows, every expert's output and their sum to bf16: three half steps in the 2-norm, ours one
+    assert (other - mine).norm() <= 4 * 2.0 ** -8 * mine.norm()
+
+
+@gpu
+def test_refusals():
+    x, wg, bg, lw, k, _, _ = small()
+    bad = [dict(x=x.float()), dict(x=x[0]), dict(wg=wg[:, :4]), dict(bg=bg[:4]), dict(bg=bg.double()), dict(bg=bg.repeat_interleave(2)[::2]), dict(k=0), dict(k=9),
+           dict(x=x[:, :64].contiguous()), dict(wg=wg.cpu()), dict(bg=bg.cpu())]
+    for change in bad:
+        a = {"x": x, "wg": wg, "bg": bg, "lw": lw, "k": k, **change}
+        with pytest.raises(ValueError):
+            tb.moe_layer_tokens(a["x"], a["wg"], a["bg"], a["lw"], a["k"])
+    with pytest.raises(NotImplementedError):
+        tb.moe_layer_tokens(x.repeat(4, 1), wg, bg, lw, k)                                               # 20 tokens
+    import dataclasses
+    plain = dataclasses.replace(lw, w1=tb.wrap_torch_tensor(torch.zeros(8, 64, 192, device="cuda", dtype=torch.uint8), dtype=tb.FP4))
+    with pytest.raises(NotImplementedError):
+        tb.moe_layer_tokens(x, wg, bg, plain, k)
+    with pytest.raises(ValueError):
+        tb.moe_layer_tokens(x, wg, bg, dataclasses.replace(lw, b2=lw.b2[:, :64]), k)
+
+
+def test_refuses_cpu_tensors():
+    with pytest.raises(ValueError):
+        tb.moe_layer_tokens(torch.zeros(1, 32, dtype=torch.bfloat16), None, None, None, 1)
+    with pytest.raises(ValueError):
+        tb.moe_layer_tokens(torch.zeros(1, 32), None, None, None, 1)
+
+
+def test_refusals_of_the_c_entry_point():
+    import ctypes
+    from triton_b200 import _lib
+    lib = _lib.load()
+    assert lib.moe_layer_tokens(None, None) == 1 and b"NULL" in lib.moe_last_error()
+    assert lib.moe_layer_tokens_workspace_bytes(None) == 0
+    blank = (ctypes.c_uint8 * 512)()                           # all sizes zero
+    assert lib.moe_layer_tokens(ctypes.addressof(blank), None) == 1 and b"positive" in lib.moe_last_error()

@@ -871,22 +871,24 @@ int64_t lr_pair_clusters(int s) {
 // 128 bytes, and draining the accumulator about as much as 2.6 rows a token.
 PairPlan lr_pair_plan(int64_t T, int K, int N) {
   PairPlan best = {};
-  const int64_t pairs = lr_pair_clusters(1), KT = cdiv64(K, BLOCK_K), tiles_n = cdiv64(N, 256);
+  const int64_t KT = cdiv64(K, BLOCK_K), tiles_n = cdiv64(N, 256);
+  int64_t side[LP_MAX_SPLITS + 1];                            // clusters of so many pairs that run side by side
+  for (int s = 1; s <= LP_MAX_SPLITS; ++s) side[s] = lr_pair_clusters(s);
   double least = 0.0;
   const int64_t fewest = cdiv64(T, LR_MAX_TB);
-  for (int64_t nb = fewest; nb <= 2 * fewest + 6; ++nb) {
+  for (int64_t nb = fewest; nb <= fewest + 8; ++nb) {
     int64_t tb = cdiv64(cdiv64(T, nb), 32) * 32;
     if (tb < 64) tb = 64;
     const int64_t blocks = cdiv64(T, tb), tiles = tiles_n * blocks;
     int64_t s = tb > 416 ? 1 : KT / 4 < LP_MAX_SPLITS ? KT / 4 : LP_MAX_SPLITS;       // (a split's sums are tb x 128 fp32 in shared memory)
-    while (s > 1 && tiles > lr_pair_clusters((int)s)) --s;
+    while (s > 1 && tiles > side[s]) --s;
     if (s < 1) s = 1;
-    const double rounds = (double)cdiv64(tiles, lr_pair_clusters((int)s));
+    const double rounds = (double)cdiv64(tiles, side[s]);
     const double cost = rounds * ((double)cdiv64(KT, s) * (128 + tb / 2) + 2.6 * tb);
     if (best.tb == 0 || cost < least) {
       least = cost;
       best.tb = (int)tb; best.blocks = (int)blocks; best.splits = (int)s; best.tiles_n = (int)tiles_n;
-      best.clusters = (int)(s > 1 || tiles < pairs ? tiles : pairs);
+      best.clusters = (int)(s > 1 || tiles < side[1] ? tiles : side[1]);
     }
   }
   best.mmas = best.tb > 256 ? 2 : 1;
