@@ -13,6 +13,7 @@
 // above.
 #include "gemm_pair_common.cuh"
 #include <cuda_fp16.h>
+#include <atomic>
 #include <type_traits>
 
 namespace {
@@ -240,6 +241,14 @@ __device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, 
   sts128(to + lo + 128, l[1]);
 }
 
+// whether the word at this place is zero in the first n CTAs of the cluster (a lane asks one of them: one after the other they took 2 us)
+__device__ __forceinline__ bool cluster_fine(uint32_t at, int n) {
+  uint32_t v = 0;
+  const int lane = threadIdx.x & 31;
+  if (lane < n)
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(at), "r"(lane) : "memory");
+  return __all_sync(0xFFFFFFFFu, v == 0);
+}
 // The shares of k of a cluster's CTAs meet, in their order: sums [token][128 outputs] at `at` in the shared memory of the CTAs step * r + base, r < S <=
 // MOST.  Tokens t0 .. t1 of the block for outputs n0 on; four outputs a thread, U of those and all shares on their way at a time (one share after the other
 // the sums of 300 tokens took 6 us).
@@ -251,7 +260,12 @@ __device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, i
   for (int r = 0; r < MOST; ++r)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from[r]) : "r"(at), "r"(step * (uint32_t)min(r, S - 1) + base));
   for (int i0 = threadIdx.x; i0 < (t1 - t0) * 32; i0 += U * blockDim.x) {
-    float q[U][MOST][4];
+    float q[U][MOST][4], bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias) {                                             // (a thread's items are a multiple of 32 apart: the same outputs)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + (i0 & 31) * 4 + j < p.N) bias[j] = load_bias(p.bias, p.bias_dtype, n0 + (i0 & 31) * 4 + j);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = min(i0 + u * (int)blockDim.x, (t1 - t0) * 32 - 1);
@@ -273,8 +287,7 @@ __device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, i
 #pragma unroll
         for (int r = 1; r < MOST; ++r)
           if (r < S) v += q[u][r][j];
-        if (p.bias && n + j < p.N) v += load_bias(p.bias, p.bias_dtype, n + j);
-        o[j] = from_f32<T16>(v);
+        o[j] = from_f32<T16>(v + bias[j]);
       }
       if (vec) {
         *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(o);
@@ -513,12 +526,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
   }
   __syncthreads();
   if (S > 1) cluster_sync_all();
-  bool ok = true;
-  for (int r = 0; r < S; ++r) {
-    uint32_t v;
-    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(smem_u32(&s_abort)), "r"(r) : "memory");
-    ok = ok && v == 0;
-  }
+  const bool ok = cluster_fine(smem_u32(&s_abort), S);
   if (ok) cluster_sums<T16, LS_MAX_SPLITS, 2>(p, sbase, S, 1u, 0u, row0, rows * rank / S, rows * (rank + 1) / S, n0);
   if (S > 1) cluster_sync_all();                              // no CTA leaves while its sums are read
   if (warp == 1) {
@@ -755,13 +763,7 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
   cluster_sync_all();
   if (S > 1) {
     // ---- the splits' sums meet, in their order: each CTA takes a share of the tokens of its half of the outputs ----
-    auto remote = [&](uint32_t at, uint32_t r) {
-      uint32_t v;
-      asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}" : "=r"(v) : "r"(at), "r"(r) : "memory");
-      return v;
-    };
-    bool ok = true;
-    for (int r = 0; r < 2 * S; ++r) ok = ok && remote(smem_u32(&s_abort), (uint32_t)r) == 0;
+    const bool ok = cluster_fine(smem_u32(&s_abort), 2 * S);
     if (ok && tile0 < tile1) {
       const int block = tile0 / pl.tiles_n, n0 = (tile0 - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
       const int64_t row0 = (int64_t)block * TB;
@@ -919,6 +921,18 @@ int lr_check(const MoeLoraArgs* a) {
   return MOE_OK;
 }
 
+// allows a kernel its dynamic shared memory, once per device (a microsecond of every call otherwise)
+int lr_allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  MOE_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return MOE_OK;
+  MOE_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return MOE_OK;
+}
+template <typename K> int lr_allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) { return lr_allow_smem((const void*)kernel, bytes, done); }
+
 template <typename T16> int lr_shrink(const LoraParams& p, const ShrinkPlan& sp, cudaStream_t st) {
   const dim3 grid((unsigned)cdiv64(p.T, 8 * sp.nb), (unsigned)(p.max_pieces + (p.list_tb > 0 ? 1 : 0)), (unsigned)(sp.places * sp.parts));
   if (sp.nb == 1) MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 1>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
@@ -933,7 +947,8 @@ template <typename T16> int lr_stream(const LoraParams& p, const MoeLoraArgs& a,
   CUtensorMap w_map, x_map;
   if (int rc = lr_map(a.w_t, a.N, a.K, a.ld_w, LR_TILE_N, f16, &w_map)) return rc;
   if (int rc = lr_map(a.x, a.T, a.K, a.ld_x, pl.tb, f16, &x_map)) return rc;
-  MOE_CHECK_CUDA(cudaFuncSetAttribute(lora_stream_kernel<T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = lr_allow_smem(lora_stream_kernel<T16>, 112 * 1024, allowed)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cdiv64(p.N, LR_TILE_N), (unsigned)cdiv64(p.T, pl.tb), (unsigned)pl.splits);
   cfg.blockDim = dim3(LS_THREADS);
@@ -956,7 +971,8 @@ template <typename T16> int lr_pair(const LoraParams& p, const MoeLoraArgs& a, c
   CUtensorMap w_map, x_map;
   if (int rc = lr_map(a.w_t, a.N, a.K, a.ld_w, LR_TILE_N, f16, &w_map)) return rc;
   if (int rc = lr_map(a.x, a.T, a.K, a.ld_x, pl.tb / pl.mmas / 2, f16, &x_map)) return rc;
-  MOE_CHECK_CUDA(cudaFuncSetAttribute(lora_pair_kernel<T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = lr_allow_smem(lora_pair_kernel<T16>, 225 * 1024, allowed)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(pl.clusters * 2 * pl.splits));
   cfg.blockDim = dim3(LP_THREADS);

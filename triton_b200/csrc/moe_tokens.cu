@@ -21,6 +21,7 @@
 #include "gemm_tc_common.cuh"
 #include "topk_select.cuh"
 #include <cuda_fp16.h>
+#include <atomic>
 #include <type_traits>
 
 namespace {
@@ -784,11 +785,7 @@ TokensWorkspace mt_workspace(const MoeTokensArgs& a) {
 
 // the shared memory that is left for the ring, whole stages
 constexpr int MT_SMEM = 232448;
-template <int NBLK> int mt_static_smem() {
-  cudaFuncAttributes at;
-  if (cudaFuncGetAttributes(&at, moe_tokens_kernel<NBLK>) != cudaSuccess) return MT_SMEM;
-  return (int)at.sharedSizeBytes;
-}
+template <int NBLK> constexpr int mt_static_smem() { return (int)(sizeof(TokensShared) + 2 * MT_SHARES * 8 * NBLK * MT_RED_LD * 4) + 64; }
 
 int mt_check(const MoeTokensArgs* a) {
   MOE_CHECK_ARG(a, "moe_layer_tokens: NULL argument");
@@ -828,7 +825,15 @@ template <int NBLK> int mt_launch(TokensParams& p, const TokensMaps& maps, cudaS
     return MOE_ERR_UNSUPPORTED;
   }
   const int smem = p.tok_bytes + p.stages * MT_STAGE_BYTES + 128;
-  MOE_CHECK_CUDA(cudaFuncSetAttribute(moe_tokens_kernel<NBLK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // once per device (a microsecond of every call otherwise)
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  MOE_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev >= 64 || !(allowed.load(std::memory_order_acquire) & bit)) {
+    MOE_CHECK_CUDA(cudaFuncSetAttribute(moe_tokens_kernel<NBLK>, cudaFuncAttributeMaxDynamicSharedMemorySize, MT_SMEM - mt_static_smem<NBLK>()));
+    if (dev < 64) allowed.fetch_or(bit, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)moe_sm_count());
   cfg.blockDim = dim3(MT_THREADS);

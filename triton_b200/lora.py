@@ -2,6 +2,7 @@
 
 The reference's `matmul` multiplies the rows of a ragged batch by their group's matrix (matmul.py:245-766); serving fine-tuned models puts one shared
 matrix under all rows and a small product of two thin matrices, another per request, on top.  `matmul_lora` does both in two kernels."""
+import itertools
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -22,16 +23,13 @@ class LoraAdapters:
     first: torch.Tensor     # int32 [adapters + 1]
     scale: torch.Tensor     # fp32 [adapters]
     ranks: tuple[int, ...]
+    max_pieces: int         # of one adapter
     d_in: int
     d_out: int
 
     @property
     def n_adapters(self):
         return len(self.ranks)
-
-    @property
-    def max_pieces(self):
-        return max((-(-r // PIECE) for r in self.ranks), default=0)
 
 
 def prepare_lora_adapters(a: Sequence[torch.Tensor], b: Sequence[torch.Tensor], scale: Sequence[float]) -> LoraAdapters:
@@ -50,21 +48,25 @@ def prepare_lora_adapters(a: Sequence[torch.Tensor], b: Sequence[torch.Tensor], 
                              f"expected [{d_in}, r] x [r, {d_out}] in {dtype} on {device}")
         if not 1 <= r <= MAX_RANK:
             raise ValueError(f"prepare_lora_adapters: adapter {i} has rank {r}; ranks are 1 to {MAX_RANK}")
-        if not bool(torch.isfinite(bi).all()):
-            raise ValueError(f"prepare_lora_adapters: b of adapter {i} has values that are not finite")
     ranks = tuple(ai.shape[1] for ai in a)
     pieces = [-(-r // PIECE) for r in ranks]
-    first = [sum(pieces[:i]) for i in range(len(pieces) + 1)]
+    first = [0, *itertools.accumulate(pieces)]
     rows, groups = -(-d_in // 8) * 8, -(-d_out // 128) * 16
-    pa = torch.zeros((first[-1] * PIECE, rows), dtype=dtype, device=device)
-    pb = torch.zeros((first[-1], groups, 2, 8, 8), dtype=dtype, device=device)
-    for ai, bi, p0, n, r in zip(a, b, first, pieces, ranks):
-        pa[p0 * PIECE:p0 * PIECE + r, :d_in] = ai.t()
-        padded = torch.zeros((n * PIECE, groups * 8), dtype=dtype, device=device)
-        padded[:r, :d_out] = bi
-        pb[p0:p0 + n] = padded.view(n, 2, 8, groups, 8).permute(0, 3, 1, 4, 2)
+
+    def stacked(parts, width, padded):                         # ranks one below the other, each adapter's up to a multiple of 16
+        fill = {n: torch.zeros((n, width), dtype=dtype, device=device) for n in {-r % PIECE for r in ranks}}
+        out = torch.zeros((first[-1] * PIECE, padded), dtype=dtype, device=device)
+        out[:, :width] = torch.cat([t for part, r in zip(parts, ranks) for t in (part, fill[-r % PIECE])])
+        return out
+
+    pa = stacked([ai.t() for ai in a], d_in, rows)
+    pb = stacked(b, d_out, groups * 8)
+    if not bool(torch.isfinite(pb).all()):
+        wrong = [i for i, bi in enumerate(b) if not bool(torch.isfinite(bi).all())]
+        raise ValueError(f"prepare_lora_adapters: b of adapters {wrong} has values that are not finite")
+    pb = pb.view(first[-1], 2, 8, groups, 8).permute(0, 3, 1, 4, 2).contiguous()
     return LoraAdapters(pa, pb, torch.tensor(first, dtype=torch.int32, device=device),
-                        torch.tensor([float(s) for s in scale], dtype=torch.float32, device=device), ranks, d_in, d_out)
+                        torch.tensor([float(s) for s in scale], dtype=torch.float32, device=device), ranks, max(pieces), d_in, d_out)
 
 
 def prepare_projection_weight(w: torch.Tensor) -> torch.Tensor:
