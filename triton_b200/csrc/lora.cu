@@ -34,6 +34,7 @@ struct LoraParams {
   int32_t* list; int list_tb;                          // of every block of list_tb tokens [LR_LIST]: how many adapters, how many pieces, the adapters
   int32_t* status;
 };
+constexpr int LR_MAX_PARTS = 4;
 constexpr int LR_MAX_TB = 512, LR_LIST = LR_MAX_TB + 4;
 
 // ---- shrink ----------------------------------------------------------------------------------------------------
@@ -301,12 +302,12 @@ __device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, i
 }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------
-constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-5 epilogue, 6-9 adapters
+constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-9 adapters and then epilogue
 constexpr int LS_MAX_STAGES = 8, LS_MAX_TB = 64, LS_MAX_SPLITS = 6;
 
 struct StreamPlan { int tb, splits, stages, smem; };           // tokens of a block, cluster, ring of k steps, bytes
 
-__device__ __forceinline__ void adapter_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void adapter_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Single tokens have an adapter each, and an MMA for one of them in 64 columns would be 63 parts zeros that somebody writes: here the second product is
 // made on CUDA cores beside the first.  A thread has an output; 16 ranks of it are 32 bytes of B.
@@ -394,25 +395,13 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     if (!ok)
       for (uint32_t w = 0; w < (1u << 16) && !mbar_test(ACC, 0); ++w) __nanosleep(64);
     __syncwarp();
-  } else if (warp < 6) {
-    // ================================= accumulator to shared memory ==================================================
-    if (__all_sync(0xFFFFFFFFu, mbar_wait(ACC, 0, ctl, 1103))) {
-      tc_fence_after();
-      const int qd = warp & 3;
-      for (int c0 = 0; c0 < TB; c0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem + (uint32_t)c0 + ((uint32_t)(qd * 32) << 16), v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c0 + j) * LR_TILE_N + qd * 32 + lane] = __uint_as_float(v[j]);
-      }
-    }
-    tc_fence_before();
   } else {
     // ================================= adapters ================================================================
-    const int tid = threadIdx.x - 192;                        // output n0 + tid
-    for (int t = 0; t < TB; ++t) extra[t * LR_TILE_N + tid] = 0.0f;
-    if (tid < TB) {
+    // two teams of four warps, one for the even tokens and one for the odd
+    const int tid = (threadIdx.x - 64) & 127, team = (warp - 2) >> 2;         // output n0 + tid
+    const unsigned long long mine_of = 0x5555555555555555ull << team;
+    for (int t = team; t < TB; t += 2) extra[t * LR_TILE_N + tid] = 0.0f;
+    if (team == 0 && tid < TB) {
       const int a = tid < rows && p.indx ? p.indx[row0 + tid] : -1;
       s_idx[tid] = a >= 0 && a < p.n_adapters ? a : -1;
     }
@@ -457,7 +446,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
       l = lo;
       i = g - s_from[lo];
     };
-    for (int j = tid; j < n_mine; j += 128) {
+    for (int j = tid + 128 * team; j < n_mine; j += 256) {
       int l, i;
       find(j, l, i);
       l2_hint(b + (int64_t)(s_first[l] + i) * p.NP * 32, LR_PIECE_BYTES);
@@ -466,12 +455,12 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     int j = -1, my_l = 0, my_i = 0, l = 0, i = 0, t = 0;      // a lane knows one piece of every 32
     unsigned long long mask = 0;
     auto advance = [&]() {                                    // to the next token of a piece; false behind the last
-      if (mask == 0) {
+      while (mask == 0) {
         if (++j >= n_mine) return false;
         if ((j & 31) == 0 && j + lane < n_mine) find(j + lane, my_l, my_i);
         l = __shfl_sync(0xFFFFFFFFu, my_l, j & 31);
         i = __shfl_sync(0xFFFFFFFFu, my_i, j & 31);
-        mask = s_mask[l];
+        mask = s_mask[l] & mine_of;
       }
       t = __ffsll((long long)mask) - 1;
       mask &= mask - 1;
@@ -479,50 +468,55 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     };
     const float* ranks = p.t + row0 * p.ld_t + (lane & 15);   // a lane holds one of the sixteen ranks of a token
     bool more = advance();
-    while (more) {
-      constexpr int U = 4;                                    // everything of four pairs is asked for before the first is taken on
-      uint4 w[U][2];
-      float r[U][4];
-      int at[U], rest[U];
+    // four pairs on their way: as one is taken on, the next takes its place
+    constexpr int U = 4;
+    uint4 w[U][2];
+    float r[U][4];
+    int at[U], rest[U];
+    auto ask = [&](int u) {
+      at[u] = -1;
+      if (!more) return;
+      const uint4* src = reinterpret_cast<const uint4*>(b + (int64_t)(s_first[l] + i) * p.NP * 32);
+      w[u][0] = src[0];
+      w[u][1] = src[8];
+      at[u] = t;
+      rest[u] = t * (int)p.ld_t + i * LR_PIECE;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        at[u] = -1;
-        rest[u] = 0;
-        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+      for (int q = 0; q < LR_MAX_PARTS; ++q) r[u][q] = q < p.t_parts ? ranks[q * p.t_part_stride + rest[u]] : 0.0f;
+      more = advance();
+    };
 #pragma unroll
-        for (int q = 0; q < 4; ++q) r[u][q] = 0.0f;
-        if (more) {
-          const uint4* src = reinterpret_cast<const uint4*>(b + (int64_t)(s_first[l] + i) * p.NP * 32);
-          w[u][0] = src[0];
-          w[u][1] = src[8];
-          at[u] = t;
-          rest[u] = t * (int)p.ld_t + i * LR_PIECE;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < p.t_parts) r[u][q] = ranks[q * p.t_part_stride + rest[u]];
-          more = advance();
-        }
-      }
+    for (int u = 0; u < U; ++u) ask(u);
+    while (at[0] >= 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (at[u] < 0) break;
-        float mine = (r[u][0] + r[u][1]) + (r[u][2] + r[u][3]);
-        for (int q = 4; q < p.t_parts; ++q) mine += ranks[q * p.t_part_stride + rest[u]];
+        const float mine = (r[u][0] + r[u][1]) + (r[u][2] + r[u][3]);
         const T16* e = reinterpret_cast<const T16*>(&w[u][0]);
         float v = 0.0f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) v = fmaf(__shfl_sync(0xFFFFFFFFu, mine, j), to_f32<T16>(e[j]), v);
         extra[at[u] * LR_TILE_N + tid] += v;
+        ask(u);
       }
     }
-  }
-  __syncthreads();
-  // the adapters' share on top of the product's
-  for (int i = threadIdx.x; i < rows * 32; i += LS_THREADS) {
-    float4 v = reinterpret_cast<float4*>(part)[i];
-    const float4 e = reinterpret_cast<const float4*>(extra)[i];
-    v.x += e.x; v.y += e.y; v.z += e.z; v.w += e.w;
-    reinterpret_cast<float4*>(part)[i] = v;
+    // ================================= accumulator and adapters' share to shared memory ==================================
+    adapter_bar();
+    if (__all_sync(0xFFFFFFFFu, mbar_wait(ACC, 0, ctl, 1103))) {
+      tc_fence_after();
+      const int qd = warp & 3;                                // the lanes of tensor memory that a warp reaches
+      for (int c0 = 16 * team; c0 < TB; c0 += 32) {
+        uint32_t v[16];
+        tmem_ld16(tmem + (uint32_t)c0 + ((uint32_t)(qd * 32) << 16), v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int o = (c0 + j) * LR_TILE_N + qd * 32 + lane;
+          part[o] = __uint_as_float(v[j]) + extra[o];
+        }
+      }
+    }
+    tc_fence_before();
   }
   __syncthreads();
   if (S > 1) cluster_sync_all();
@@ -819,7 +813,7 @@ ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   // shares of k while the blocks that have something to do, a quarter of them say, are fewer than the SMs
   const int64_t blocks = cdiv64(T, 8 * s.nb) * max_pieces * (s.nb == 1 && s.places > 2 ? s.places / 2 : 1);
   int parts = 1;
-  while (parts < 4 && blocks * parts <= moe_sm_count() && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
+  while (parts < LR_MAX_PARTS && blocks * parts <= moe_sm_count() && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
   s.parts = parts;
   return s;
 }
