@@ -43,6 +43,10 @@ constexpr int MT_MAX_STAGES = 12;
 constexpr int MT_COUNTERS = 256;          // words of each of the three counter arrays
 constexpr int MT_ROUTER_THREADS = 256;
 
+// x / d by a product, right for x d < 2^40 and x < 2^24 d: a division by a number known at launch only costs some 20 instructions
+struct Div { uint32_t d; uint64_t m; };
+__device__ __forceinline__ int operator/(int x, const Div& v) { return (int)(((uint64_t)(uint32_t)x * v.m) >> 40); }
+
 struct TokensParams {
   const void* x; int x_dtype; int64_t ld_x;
   int T, d, ff, E, k;
@@ -55,6 +59,7 @@ struct TokensParams {
   float* logits; float* xmax;
   int32_t* done1; int32_t* done2; uint32_t* hmax;       // units of fc1 per expert, stages of fc2 per 32 columns, largest |h| per entry
   float* h; float* part;
+  Div by_ctas, by_units1, by_units2, by_steps2;        // CTAs, units of an expert in fc1 and fc2, stages of a unit of fc2
   int stages, tok_bytes;                // of the ring; shared memory of the staged tokens
   int32_t* status;
 };
@@ -224,7 +229,7 @@ __device__ __forceinline__ void mbar_wait_short(uint32_t bar, uint32_t parity, c
   while (!mbar_try(bar, parity))
     if ((++tries & 1023u) == 0 && mbar_expired(tries, ctl, code)) break;
 }
-// named barriers: 1 consumers, 2 epilogue
+// named barriers: 1 consumers, 2 epilogue, 3 all but those that stage tokens
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int MT_BOTH = MT_CONSUMERS + MT_EPILOGUE;
 
@@ -233,11 +238,10 @@ struct TokensShared {                   // beside ring, staged tokens and partia
   uint64_t sums[2], taken[2];           // a buffer of sums is complete, has been read
   int abort;
   int n_active;
-  int counts[8];
   int act[MT_MAX_EXPERTS];              // active experts in ascending order
   uint16_t rank[MT_MAX_EXPERTS];        // place of an expert in that list
-  uint16_t tokens[MT_MAX_EXPERTS];      // its tokens, a bit each
-  alignas(16) uint8_t slot[MT_MAX_EXPERTS][MT_MAX_TOKENS];     // which pick of the token it is, 255: none
+  alignas(16) uint32_t tokens[MT_MAX_EXPERTS];     // its tokens, a bit each
+  uint8_t slot[MT_MAX_EXPERTS][MT_MAX_TOKENS];     // which pick of its tokens it is
   uint8_t who[MT_MAX_EXPERTS][MT_MAX_TOKENS];      // its tokens one behind the other
   uint8_t sel[MT_MAX_TOKENS][MT_MAX_K];
   float gate[MT_MAX_TOKENS][MT_MAX_K];
@@ -270,7 +274,10 @@ __device__ __forceinline__ void select_token(const TokensParams& p, TokensShared
     const float w = expf(v - first);
     sum += w;
     if (lane == j) mine = w;
-    if (lane == 0) s.sel[t][j] = (uint8_t)e;
+    if (lane == 0) {
+      s.sel[t][j] = (uint8_t)e;
+      atomicOr(&s.tokens[e], 1u << t);
+    }
   }
   if (lane < p.k) s.gate[t][lane] = __fdiv_rn(mine, sum);
 }
@@ -378,46 +385,51 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     s.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (threadIdx.x < MT_MAX_EXPERTS) *reinterpret_cast<uint4*>(s.slot[threadIdx.x]) = make_uint4(~0u, ~0u, ~0u, ~0u);
-  if (warp < p.T) select_token(p, s, warp, lane);
-  else if (NBLK == 1 && warp >= 8 && warp - 8 < p.T) stage_x(p, s, NBLK, toks, warp - 8);
+  if (threadIdx.x < MT_MAX_EXPERTS) s.tokens[threadIdx.x] = 0;
   __syncthreads();
-  if (threadIdx.x < p.T * p.k) {
-    const int t = threadIdx.x / p.k, j = threadIdx.x - t * p.k;
-    s.slot[s.sel[t][j]][t] = (uint8_t)j;
-  }
-  __syncthreads();
-  {
-    uint32_t mask = 0;
-    const int e = threadIdx.x;
-    if (e < MT_MAX_EXPERTS) {
+  // Half of the consumers stage the tokens while the others select; the weights are on their way before the tokens are there.
+  if (warp >= MT_WARPS / 2 && warp < MT_WARPS) {
+    for (int t = warp - MT_WARPS / 2; t < p.T; t += MT_WARPS / 2) stage_x(p, s, NBLK, toks, t);
+  } else {
+    constexpr int OTHERS = MT_THREADS - MT_CONSUMERS / 2;
+    if (warp < MT_WARPS / 2)
+      for (int t = warp; t < p.T; t += MT_WARPS / 2) select_token(p, s, t, lane);
+    bar_sync(3, OTHERS);
+    if (warp == MT_WARPS) {             // the list of active experts, eight a lane
+      uint32_t on = 0;
 #pragma unroll
-      for (int t = 0; t < MT_MAX_TOKENS; ++t)
-        if (s.slot[e][t] != 0xFF) {
-          s.who[e][__popc(mask)] = (uint8_t)t;
-          mask |= 1u << t;
-        }
-      s.tokens[e] = (uint16_t)mask;
+      for (int h = 0; h < 2; ++h) {
+        const uint4 v = *reinterpret_cast<const uint4*>(&s.tokens[lane * 8 + h * 4]);
+        on |= ((v.x ? 1u : 0u) | (v.y ? 2u : 0u) | (v.z ? 4u : 0u) | (v.w ? 8u : 0u)) << (4 * h);
+      }
+      int at = __popc(on);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int q = __shfl_up_sync(0xFFFFFFFFu, at, o);
+        if (lane >= o) at += q;
+      }
+      if (lane == 31) s.n_active = at;
+      for (at -= __popc(on); on; on &= on - 1, ++at) {
+        const int e = lane * 8 + __ffs(on) - 1;
+        s.act[at] = e;
+        s.rank[e] = (uint16_t)at;
+      }
+    } else if (threadIdx.x < p.T * p.k) {
+      const int t = threadIdx.x / p.k, j = threadIdx.x - t * p.k, e = s.sel[t][j];
+      s.slot[e][t] = (uint8_t)j;
+      s.who[e][__popc(s.tokens[e] & ((1u << t) - 1u))] = (uint8_t)t;
     }
-    const uint32_t live = __ballot_sync(0xFFFFFFFFu, mask != 0);
-    if (e < MT_MAX_EXPERTS && lane == 0) s.counts[warp] = __popc(live);
-    __syncthreads();
-    if (e < MT_MAX_EXPERTS) {
-      int at = __popc(live & ((1u << lane) - 1u));
-      for (int w = 0; w < warp; ++w) at += s.counts[w];
-      if (mask) { s.act[at] = e; s.rank[e] = (uint16_t)at; }
-      if (e == MT_MAX_EXPERTS - 1) s.n_active = at + (mask ? 1 : 0);
-    }
-    __syncthreads();
+    bar_sync(3, OTHERS);
   }
+  if (warp < MT_WARPS) bar_sync(1, MT_CONSUMERS);
 
   const int A = s.n_active, G = gridDim.x, c = blockIdx.x;
   const int KT1 = (p.d + 127) >> 7, KT2 = (p.ff + 127) >> 7, KS1 = (KT1 + MT_STAGE_KT - 1) / MT_STAGE_KT, KS2 = (KT2 + MT_STAGE_KT - 1) / MT_STAGE_KT;
   const int NB1 = 2 * p.ff / MT_UNIT, NB2 = p.d / MT_UNIT, NT1 = (2 * p.ff + 127) >> 7, NT2 = (p.d + 127) >> 7;
   const int U1 = A * NB1;
   const int S2 = A * NB2 * KS2;                              // (times the CTAs it stays below 2^31: 2^19 * 148)
-  const int u_begin = U1 * c / G, u_end = U1 * (c + 1) / G, s_begin = S2 * c / G, s_end = S2 * (c + 1) / G;
-  const int first2 = s_begin / KS2, n1 = u_end - u_begin, n2 = s_end > s_begin ? (s_end - 1) / KS2 - first2 + 1 : 0;      // units here
+  const int u_begin = U1 * c / p.by_ctas, u_end = U1 * (c + 1) / p.by_ctas, s_begin = S2 * c / p.by_ctas, s_end = S2 * (c + 1) / p.by_ctas;
+  const int first2 = s_begin / p.by_steps2, n1 = u_end - u_begin, n2 = s_end > s_begin ? (s_end - 1) / p.by_steps2 - first2 + 1 : 0;      // units here
 
   if (warp == MT_BOTH / 32) {
     // ================================= weights =================================================================
@@ -441,10 +453,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     };
     int m = 0;
     // units [from, from + units) of a product, their stages from js0 in the first to js1 in the last
-    auto product = [&](const CUtensorMap* v, const CUtensorMap* sc, const CUtensorMap* vt, const CUtensorMap* st, int NB, int NT, int KT, int KS, int from,
+    auto product = [&](const CUtensorMap* v, const CUtensorMap* sc, const CUtensorMap* vt, const CUtensorMap* st, int NB, const Div& by, int NT, int KT, int KS, int from,
                        int units, int js0, int js1) {
       const uint32_t whole = MT_STAGE_KT * MT_UNIT * 68, tail = (uint32_t)((KT - (KS - 1) * MT_STAGE_KT) * MT_UNIT * 68);
-      int place = from / NB, nb = from - place * NB;
+      int place = from / by, nb = from - place * NB;
 #pragma unroll 1
       for (int i = 0; i < units && ok; ++i, ++m) {
         const int tile = (s.act[place] * NT + (nb >> 2)) * KT, end = i + 1 == units ? js1 : KS;
@@ -456,8 +468,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         if (++nb == NB) { nb = 0; ++place; }
       }
     };
-    product(&maps.v1, &maps.s1, &maps.v1t, &maps.s1t, NB1, NT1, KT1, KS1, u_begin, n1, 0, KS1);
-    product(&maps.v2, &maps.s2, &maps.v2t, &maps.s2t, NB2, NT2, KT2, KS2, first2, n2, s_begin - first2 * KS2, s_end - (first2 + n2 - 1) * KS2);
+    product(&maps.v1, &maps.s1, &maps.v1t, &maps.s1t, NB1, p.by_units1, NT1, KT1, KS1, u_begin, n1, 0, KS1);
+    product(&maps.v2, &maps.s2, &maps.v2t, &maps.s2t, NB2, p.by_units2, NT2, KT2, KS2, first2, n2, s_begin - first2 * KS2, s_end - (first2 + n2 - 1) * KS2);
     if (!ok) __nanosleep(500000);                             // copies in flight land before the block's shared memory goes
     return;
   }
@@ -465,7 +477,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   if (warp >= MT_WARPS) {
     // ================================= epilogue ================================================================
     const int tid = threadIdx.x - MT_CONSUMERS;
-    int a = u_begin / NB1, nb = u_begin - a * NB1;            // of the unit
+    int a = u_begin / p.by_units1, nb = u_begin - a * NB1;    // of the unit
     const int i = tid & 15;
     // the bias of a unit is asked for while the one before is at work: its way from memory is longer than a unit's
     float bias[2] = {0.0f, 0.0f};
@@ -541,7 +553,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     int have = -1, changes = -1;
 #pragma unroll 1
     for (int m = n1; m < n1 + n2; ++m) {
-      const int u = first2 + m - n1, e = s.act[u / NB2], n = __popc(s.tokens[e]), lane_row = tid & 31;
+      const int u = first2 + m - n1, place = u / p.by_units2, e = s.act[place], n = __popc(s.tokens[e]), lane_row = tid & 31;
       if (e != have) { have = e; ++changes; }
       mbar_wait_short(SUMS(m & 1), (m >> 1) & 1u, ctl, 1005);
       for (int r = tid >> 5; r < n; r += MT_EPILOGUE / 32) {
@@ -552,7 +564,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
 #pragma unroll
           for (int w = 0; w < MT_SHARES; ++w) v += s_red[m & 1][w][(n + r) * MT_RED_LD + lane_row];
         }
-        __stcg(p.part + ((int64_t)(u + c) * p.T + r) * MT_UNIT + lane_row, settle(v, p.s2, e, NT2, KT2, (u % NB2) * MT_UNIT + lane_row) * s.undo2[changes & 3][r]);
+        __stcg(p.part + ((int64_t)(u + c) * p.T + r) * MT_UNIT + lane_row, settle(v, p.s2, e, NT2, KT2, (u - place * NB2) * MT_UNIT + lane_row) * s.undo2[changes & 3][r]);
       }
       __syncwarp();
       if ((tid & 31) == 0) mbar_arrive(TAKEN(m & 1));
@@ -561,7 +573,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     for (int i = tid; i < n2; i += MT_EPILOGUE) {
       const int u = first2 + i;
       __threadfence();
-      atomicAdd(p.done2 + u % NB2, min(s_end, (u + 1) * KS2) - max(s_begin, u * KS2));
+      atomicAdd(p.done2 + (u - u / p.by_units2 * NB2), min(s_end, (u + 1) * KS2) - max(s_begin, u * KS2));
     }
     return;
   }
@@ -626,18 +638,14 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     if (++ri == half) { ri = 0; rp ^= 1u; }
   };
 
-  if (NBLK == 2) {
-    if (warp < p.T) stage_x(p, s, NBLK, toks, warp);
-    bar_sync(1, MT_CONSUMERS);
-  }
   // ---- all units, fc1's and fc2's ----
   int have = -1, changes = -1;          // expert whose rows of fc2 are staged
   int n_blocks = 1;                     // of the expert's tokens as columns
-  int place = u_begin / NB1, rest = u_begin - place * NB1;   // the unit's expert in the list of active ones, its place among the expert's units
+  int place = u_begin / p.by_units1, rest = u_begin - place * NB1;   // the unit's expert in the list of active ones, its place among the expert's units
 #pragma unroll 1
   for (int m = 0; m < n1 + n2; ++m, ++rest) {
     const bool one = m < n1;
-    if (m == n1) { place = first2 / NB2; rest = first2 - place * NB2; }
+    if (m == n1) { place = first2 / p.by_units2; rest = first2 - place * NB2; }
     if (rest == (one ? NB1 : NB2)) { rest = 0; ++place; }
     const int e = s.act[place], KT = one ? KT1 : KT2;
     const int js0 = m == n1 ? s_begin - first2 * KS2 : 0, js1 = one ? KS1 : m + 1 == n1 + n2 ? s_end - (first2 + n2 - 1) * KS2 : KS2;
@@ -693,7 +701,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
 
   // ---- the selected experts' sums meet: a warp takes 32 outputs of a token as soon as all of their stages are done ----
   for (int i = warp * G + c; i < NB2 * p.T; i += MT_WARPS * G) {
-    const int t = i / NB2, nb = i - t * NB2, o = nb * MT_UNIT + lane;
+    const int t = i / p.by_units2, nb = i - t * NB2, o = nb * MT_UNIT + lane;
     float y = 0.0f;
     for (int j0 = 0; j0 < p.k; j0 += 4) {
       float v[4], b[4];
@@ -715,13 +723,19 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
       }
       wait_count(p.done2 + nb, A * KS2, ctl, 1004);
       __syncwarp();
+      // the first part and the last, most often all there are, side by side
+      float last[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] = j0 + x < p.k ? __ldcg(part[x] + (int64_t)c0[x] * p.T * MT_UNIT) : 0.0f;
+      for (int x = 0; x < 4; ++x) {
+        v[x] = j0 + x < p.k ? __ldcg(part[x] + (int64_t)c0[x] * p.T * MT_UNIT) : 0.0f;
+        last[x] = c1[x] > c0[x] ? __ldcg(part[x] + (int64_t)c1[x] * p.T * MT_UNIT) : 0.0f;
+      }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         if (j0 + x >= p.k) break;
-        for (int cc = c0[x] + 1; cc <= c1[x]; ++cc)
-          if (S2 * cc / G < S2 * (cc + 1) / G) v[x] += __ldcg(part[x] + (int64_t)cc * p.T * MT_UNIT);
+        for (int cc = c0[x] + 1; cc < c1[x]; ++cc)
+          if (S2 * cc / p.by_ctas < S2 * (cc + 1) / p.by_ctas) v[x] += __ldcg(part[x] + (int64_t)cc * p.T * MT_UNIT);
+        v[x] += last[x];
         y = fmaf(s.gate[t][j0 + x], v[x] + b[x], y);
       }
     }
@@ -825,6 +839,11 @@ template <int NBLK> int mt_launch(TokensParams& p, const TokensMaps& maps, cudaS
     return MOE_ERR_UNSUPPORTED;
   }
   const int smem = p.tok_bytes + p.stages * MT_STAGE_BYTES + 128;
+  const auto div = [](int d) { return Div{(uint32_t)d, (1ull << 40) / (uint64_t)d + 1}; };
+  p.by_ctas = div(moe_sm_count());
+  p.by_units1 = div(2 * p.ff / MT_UNIT);
+  p.by_units2 = div(p.d / MT_UNIT);
+  p.by_steps2 = div((int)cdiv64(cdiv64(p.ff, 128), MT_STAGE_KT));
   // once per device (a microsecond of every call otherwise)
   static std::atomic<uint64_t> allowed{0};
   int dev = 0;
