@@ -257,29 +257,30 @@ __device__ __forceinline__ void select_token(const TokensParams& p, TokensShared
     const int e = lane + 32 * i;
     key[i] = e < p.E ? sel_float_key(__ldcg(p.logits + t * p.E + e)) : 0u;
   }
-  float first = 0.0f, sum = 0.0f, mine = 0.0f;
+  uint32_t mine = 0u;                   // lane j's: the j-th largest and its expert
+  int expert = 0;
   for (int j = 0; j < p.k; ++j) {
-    uint32_t best = 0u;
-    int at = MT_MAX_EXPERTS;
+    uint32_t best = key[0];
+    int at = lane;
 #pragma unroll
-    for (int i = 0; i < MT_MAX_EXPERTS / 32; ++i)
-      if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+    for (int i = 1; i < MT_MAX_EXPERTS / 32; ++i)
+      if (32 * i < p.E && key[i] > best) { best = key[i]; at = lane + 32 * i; }
     const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
     const int e = __reduce_min_sync(0xFFFFFFFFu, best == top ? at : MT_MAX_EXPERTS);
 #pragma unroll
     for (int i = 0; i < MT_MAX_EXPERTS / 32; ++i)
-      if (lane + 32 * i == e) key[i] = 0u;
-    const float v = sel_key_float(top);
-    if (j == 0) first = v;
-    const float w = expf(v - first);
-    sum += w;
-    if (lane == j) mine = w;
-    if (lane == 0) {
-      s.sel[t][j] = (uint8_t)e;
-      atomicOr(&s.tokens[e], 1u << t);
-    }
+      if (32 * i < p.E && lane + 32 * i == e) key[i] = 0u;
+    if (lane == j) { mine = top; expert = e; }
   }
-  if (lane < p.k) s.gate[t][lane] = __fdiv_rn(mine, sum);
+  const float first = sel_key_float(__shfl_sync(0xFFFFFFFFu, mine, 0)), w = lane < p.k ? expf(sel_key_float(mine) - first) : 0.0f;
+  float sum = w;
+#pragma unroll
+  for (int o = MT_MAX_K / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (lane < p.k) {
+    s.sel[t][lane] = (uint8_t)expert;
+    atomicOr(&s.tokens[expert], 1u << t);
+    s.gate[t][lane] = __fdiv_rn(w, sum);
+  }
 }
 
 // staged token column col, eight k from 8 * k8 on
