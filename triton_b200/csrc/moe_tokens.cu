@@ -240,6 +240,7 @@ struct TokensShared {                   // beside ring, staged tokens and partia
   int n_active;
   int act[MT_MAX_EXPERTS];              // active experts in ascending order
   uint16_t rank[MT_MAX_EXPERTS];        // place of an expert in that list
+  uint32_t ahead[MT_MAX_EXPERTS + 1];   // by that place: time of a step of fc1 in all experts ahead (low half) and of fc2 (high half), see step_time
   alignas(16) uint32_t tokens[MT_MAX_EXPERTS];     // its tokens, a bit each
   uint8_t slot[MT_MAX_EXPERTS][MT_MAX_TOKENS];     // which pick of its tokens it is
   uint8_t who[MT_MAX_EXPERTS][MT_MAX_TOKENS];      // its tokens one behind the other
@@ -360,6 +361,32 @@ __device__ __forceinline__ void stage_h(const TokensParams& p, TokensShared& s, 
   }
 }
 
+// What a stage takes the tensor-core loop, relative to others: the columns' second block of eight costs half as much as everything else
+__device__ __forceinline__ uint32_t step_time(int n, int nblk) {
+  return nblk == 1 ? 0x10001u : (n > 8 ? 3u : 2u) + ((two_terms(n, nblk) ? 2 * n : n) > 8 ? 0x30000u : 0x20000u);
+}
+// Steps of a product, `per` an expert, are dealt out to CTAs by that time.  The CTA of a step: where the time ahead of it falls.
+template <int NBLK, int SHIFT>
+__device__ __forceinline__ int cta_of(const TokensShared& s, int step, int place, int per, int total, int G) {
+  if (NBLK == 1) return step * G / total;
+  const int ahead = (s.ahead[place] >> SHIFT) & 0xFFFF, each = ((s.ahead[place + 1] >> SHIFT) & 0xFFFF) - ahead;
+  return (ahead * per + (step - place * per) * each) * G / total;
+}
+// The first step of CTA c, by a warp: cta_of is c or more from there on
+template <int NBLK, int SHIFT>
+__device__ __forceinline__ int first_step(const TokensShared& s, int c, int per, int total, int G, const Div& by_ctas) {
+  const int time = (total * c + G - 1) / by_ctas;
+  if (NBLK == 1) return time;
+  int place = -1;                       // the last expert that begins at that time or before
+#pragma unroll
+  for (int i = 0; i < MT_MAX_EXPERTS / 32; ++i) {
+    const int a = i * 32 + (threadIdx.x & 31);
+    if (i * 32 < s.n_active) place += __popc(__ballot_sync(0xFFFFFFFFu, a < s.n_active && (int)((s.ahead[a] >> SHIFT) & 0xFFFF) * per <= time));
+  }
+  const int ahead = (s.ahead[place] >> SHIFT) & 0xFFFF, each = ((s.ahead[place + 1] >> SHIFT) & 0xFFFF) - ahead;
+  return place * per + (time - ahead * per + each - 1) / each;
+}
+
 template <int NBLK>                     // blocks of eight token columns
 __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensParams p, const __grid_constant__ TokensMaps maps) {
   extern __shared__ uint8_t smem_raw[];
@@ -397,24 +424,32 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
       for (int t = warp; t < p.T; t += MT_WARPS / 2) select_token(p, s, t, lane);
     bar_sync(3, OTHERS);
     if (warp == MT_WARPS) {             // the list of active experts, eight a lane
-      uint32_t on = 0;
+      uint32_t takes[8], on = 0, time = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 v = *reinterpret_cast<const uint4*>(&s.tokens[lane * 8 + h * 4]);
-        on |= ((v.x ? 1u : 0u) | (v.y ? 2u : 0u) | (v.z ? 4u : 0u) | (v.w ? 8u : 0u)) << (4 * h);
+      for (int i = 0; i < 8; ++i) {
+        const int n = __popc(s.tokens[lane * 8 + i]);
+        takes[i] = n ? step_time(n, NBLK) : 0u;
+        time += takes[i];
+        on += n ? 1u : 0u;
       }
-      int at = __popc(on);
+      uint32_t at = on, ahead = time;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int q = __shfl_up_sync(0xFFFFFFFFu, at, o);
-        if (lane >= o) at += q;
+        const uint32_t q = __shfl_up_sync(0xFFFFFFFFu, at, o), w = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
+        if (lane >= o) { at += q; ahead += w; }
       }
-      if (lane == 31) s.n_active = at;
-      for (at -= __popc(on); on; on &= on - 1, ++at) {
-        const int e = lane * 8 + __ffs(on) - 1;
-        s.act[at] = e;
-        s.rank[e] = (uint16_t)at;
-      }
+      if (lane == 31) { s.n_active = (int)at; s.ahead[at] = ahead; }
+      at -= on;
+      ahead -= time;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (takes[i]) {
+          s.act[at] = lane * 8 + i;
+          s.rank[lane * 8 + i] = (uint16_t)at;
+          s.ahead[at] = ahead;
+          ++at;
+          ahead += takes[i];
+        }
     } else if (threadIdx.x < p.T * p.k) {
       const int t = threadIdx.x / p.k, j = threadIdx.x - t * p.k, e = s.sel[t][j];
       s.slot[e][t] = (uint8_t)j;
@@ -428,8 +463,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   const int KT1 = (p.d + 127) >> 7, KT2 = (p.ff + 127) >> 7, KS1 = (KT1 + MT_STAGE_KT - 1) / MT_STAGE_KT, KS2 = (KT2 + MT_STAGE_KT - 1) / MT_STAGE_KT;
   const int NB1 = 2 * p.ff / MT_UNIT, NB2 = p.d / MT_UNIT, NT1 = (2 * p.ff + 127) >> 7, NT2 = (p.d + 127) >> 7;
   const int U1 = A * NB1;
-  const int S2 = A * NB2 * KS2;                              // (times the CTAs it stays below 2^31: 2^19 * 148)
-  const int u_begin = U1 * c / p.by_ctas, u_end = U1 * (c + 1) / p.by_ctas, s_begin = S2 * c / p.by_ctas, s_end = S2 * (c + 1) / p.by_ctas;
+  const int time1 = (int)(s.ahead[A] & 0xFFFF) * NB1, time2 = (int)(s.ahead[A] >> 16) * NB2 * KS2;      // (times the CTAs below 2^26: the widths' limits)
+  const int u_begin = first_step<NBLK, 0>(s, c, NB1, time1, G, p.by_ctas), u_end = c + 1 == G ? U1 : first_step<NBLK, 0>(s, c + 1, NB1, time1, G, p.by_ctas);
+  const int s_begin = first_step<NBLK, 16>(s, c, NB2 * KS2, time2, G, p.by_ctas);
+  const int s_end = c + 1 == G ? A * NB2 * KS2 : first_step<NBLK, 16>(s, c + 1, NB2 * KS2, time2, G, p.by_ctas);
   const int first2 = s_begin / p.by_steps2, n1 = u_end - u_begin, n2 = s_end > s_begin ? (s_end - 1) / p.by_steps2 - first2 + 1 : 0;      // units here
 
   if (warp == MT_BOTH / 32) {
@@ -715,9 +752,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         part[x] = nullptr;
         if (j0 + x < p.k) {
           const int e = s.sel[t][j0 + x], u = (int)s.rank[e] * NB2 + nb, r = __popc(s.tokens[e] & ((1u << t) - 1u));
-          // the CTAs whose ranges the unit's stages are in (those between with nothing to do where there are fewer stages than CTAs)
-          c0[x] = ((u * KS2 + 1) * G - 1) / S2;
-          c1[x] = ((u + 1) * KS2 * G - 1) / S2;
+          // the CTAs whose ranges the unit's first and last stage are in
+          c0[x] = cta_of<NBLK, 16>(s, u * KS2, s.rank[e], NB2 * KS2, time2, G);
+          c1[x] = cta_of<NBLK, 16>(s, u * KS2 + KS2 - 1, s.rank[e], NB2 * KS2, time2, G);
           part[x] = p.part + ((int64_t)u * p.T + r) * MT_UNIT + lane;
           if (p.b2) b[x] = load_bias(p.b2, p.b2_dtype, e * p.ld_b2 + o);
         }
@@ -734,8 +771,14 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         if (j0 + x >= p.k) break;
-        for (int cc = c0[x] + 1; cc < c1[x]; ++cc)
-          if (S2 * cc / p.by_ctas < S2 * (cc + 1) / p.by_ctas) v[x] += __ldcg(part[x] + (int64_t)cc * p.T * MT_UNIT);
+        if (c1[x] > c0[x] + 1) {
+          const int place = s.rank[s.sel[t][j0 + x]];
+          for (int q = 1, was = c0[x]; q < KS2 - 1; ++q) {
+            const int cc = cta_of<NBLK, 16>(s, (place * NB2 + nb) * KS2 + q, place, NB2 * KS2, time2, G);
+            if (cc != was && cc != c1[x]) v[x] += __ldcg(part[x] + (int64_t)cc * p.T * MT_UNIT);
+            was = cc;
+          }
+        }
         v[x] += last[x];
         y = fmaf(s.gate[t][j0 + x], v[x] + b[x], y);
       }
