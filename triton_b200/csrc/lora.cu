@@ -47,66 +47,81 @@ template <typename T16> __device__ __forceinline__ void mma_16816(float (&d)[4],
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+constexpr int SH_WARPS = 8;
+
 // Adapter of each of `rows` tokens from row0 on (-1: none, and for the rows past them) and the list of those that occur, in the order of their first
-// token.  All threads of the block call; `idx` (16-byte aligned) and `list`, block_rows (a multiple of 4) each, are in shared memory; behind a
-// barrier, with one at the end.
-__device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, int rows, int block_rows, int* idx, int* list, int* count) {
-  for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {
+// token.  All threads of the block call; `idx` and `list`, ROWS each, and `table`, 4 ROWS, are in shared memory; behind a barrier, with one at the end.
+// An adapter's first token is found through a hash table of 2 ROWS places, half of which stay free (every token with every one before it: 4 us of 512).
+template <int ROWS>
+__device__ __forceinline__ void adapters_of(const LoraParams& p, int64_t row0, int rows, int* idx, int* list, int* table, int* count) {
+  constexpr int SLOTS = 2 * ROWS, MINE = (ROWS + SH_WARPS * 32 - 1) / (SH_WARPS * 32);
+  int *key = table, *least = table + SLOTS;
+  for (int i = threadIdx.x; i < SLOTS; i += SH_WARPS * 32) { key[i] = -1; least[i] = ROWS; }
+  for (int r = threadIdx.x; r < ROWS; r += SH_WARPS * 32) {
     const int a = r < rows && p.indx ? p.indx[row0 + r] : -1;
     idx[r] = a >= 0 && a < p.n_adapters ? a : -1;
   }
   __syncthreads();
-  for (int r = threadIdx.x; r < block_rows; r += blockDim.x) {          // an adapter counts at its first token
-    bool fresh = idx[r] >= 0 && (r == 0 || idx[r - 1] != idx[r]);        // (most often runs)
-    for (int i = 0; i < r && fresh; i += 16) {                // (behind r up to the next multiple of 16, all of the block's)
-      int same = 0;
+  int at[MINE];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (i + 4 * q >= block_rows) break;
-        const int4 v = *reinterpret_cast<const int4*>(idx + i + 4 * q);
-        same |= (v.x == idx[r] && i + 4 * q < r) | (v.y == idx[r] && i + 4 * q + 1 < r) | (v.z == idx[r] && i + 4 * q + 2 < r) | (v.w == idx[r] && i + 4 * q + 3 < r);
+  for (int m = 0; m < MINE; ++m) {
+    const int r = threadIdx.x + m * SH_WARPS * 32, a = r < ROWS ? idx[r] : -1;
+    at[m] = -1;
+    if (a >= 0 && (r == 0 || idx[r - 1] != a)) {              // (most often runs)
+      uint32_t h = (uint32_t)a * 2654435761u % SLOTS;
+      for (;;) {
+        const int was = atomicCAS(key + h, -1, a);
+        if (was == -1 || was == a) break;
+        h = (h + 1) % SLOTS;
       }
-      fresh = !same;
+      atomicMin(least + h, r);
+      at[m] = (int)h;
     }
-    list[r] = fresh ? idx[r] : -1;
   }
   __syncthreads();
-  if (threadIdx.x < 32) {
+  uint32_t fresh[MINE];                                       // of the warp's 32 tokens
+#pragma unroll
+  for (int m = 0; m < MINE; ++m) {
+    const int r = threadIdx.x + m * SH_WARPS * 32;
+    fresh[m] = __ballot_sync(0xFFFFFFFFu, at[m] >= 0 && least[at[m]] == r);
+    if ((threadIdx.x & 31) == 0 && r < ROWS) key[r >> 5] = __popc(fresh[m]);      // (the keys have been read)
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < MINE; ++m) {
+    const int r = threadIdx.x + m * SH_WARPS * 32, lane = threadIdx.x & 31;
     int n = 0;
-    for (int r0 = 0; r0 < block_rows; r0 += 32) {
-      const int r = r0 + threadIdx.x, a = r < block_rows ? list[r] : -1;
-      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, a >= 0);
-      if (a >= 0) list[n + __popc(mask & ((1u << threadIdx.x) - 1u))] = a;      // (at or before where it was read)
-      n += __popc(mask);
-      __syncwarp();
-    }
-    if (threadIdx.x == 0) *count = n;
+    if (r < ROWS)
+      for (int i = 0; i < r >> 5; ++i) n += key[i];
+    if ((fresh[m] >> lane) & 1u) list[n + __popc(fresh[m] & ((1u << lane) - 1u))] = idx[r];
+    if (r == ROWS - 32) *count = n + __popc(fresh[m]);
   }
   __syncthreads();
 }
 
-constexpr int SH_WARPS = 8;
-
-// grid: (blocks of 8 NB tokens, pieces of an adapter and one for the lists, shares of k x places in the list of the block's adapters).  A block of
-// threads has one adapter of its tokens (eights), or every `places`-th (sixty-fours), and splits k over its warps: what it takes is one or two trips to
-// memory, and a warp with an adapter to itself took four times as many.
+// grid: (blocks of 8 NB tokens, pieces of an adapter, [the lists,] places in the list of the block's adapters x shares of k).  A block of threads has one
+// adapter of its tokens (eights), or every `places`-th (sixty-fours), and splits k over its warps: what it takes is one or two trips to memory, and a warp
+// with an adapter to itself took four times as many.  The blocks that take longest, the lists', come first, and those of later places, most of which find
+// no adapter, last.
 template <typename T16, int NB>
-__global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_kernel(const LoraParams p, const int places) {
-  __shared__ __align__(16) int s_idx[8 * NB], s_list[8 * NB], s_count;
-  __shared__ __align__(16) float s_sum[SH_WARPS][NB][32][4];
+__global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_kernel(const LoraParams p) {
+  __shared__ int s_idx[8 * NB], s_list[8 * NB], s_table[NB == 1 ? 1 : 32 * NB], s_count;
+  constexpr int SUM_WORDS = SH_WARPS * NB * 128, LIST_WORDS = 6 * LR_MAX_TB;
+  __shared__ __align__(16) float s_words[SUM_WORDS > LIST_WORDS ? SUM_WORDS : LIST_WORDS];
+  float (&s_sum)[SH_WARPS][NB][32][4] = *reinterpret_cast<float (*)[SH_WARPS][NB][32][4]>(s_words);
   pdl_begin();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qrow = lane >> 2, c4 = lane & 3;
-  if ((int)blockIdx.y == p.max_pieces) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qrow = lane >> 2, c4 = lane & 3, lists = p.list_tb > 0 ? 1 : 0;
+  if ((int)blockIdx.z < lists) {
     // the adapters of the product's blocks of tokens, for its kernel
-    if (blockIdx.z == 0 && (int64_t)blockIdx.x * p.list_tb < p.T) {
-      int* idx = reinterpret_cast<int*>(s_sum);
+    if (blockIdx.y == 0 && (int64_t)blockIdx.x * p.list_tb < p.T) {
+      int *idx = reinterpret_cast<int*>(s_words), *list = idx + LR_MAX_TB;
       const int64_t from = (int64_t)blockIdx.x * p.list_tb;
-      adapters_of(p, from, (int)min((int64_t)p.list_tb, (int64_t)p.T - from), p.list_tb, idx, idx + LR_MAX_TB, &s_count);
+      adapters_of<LR_MAX_TB>(p, from, (int)min((int64_t)p.list_tb, (int64_t)p.T - from), idx, list, list + LR_MAX_TB, &s_count);
       int32_t* out = p.list + (int64_t)blockIdx.x * LR_LIST;
       const int n = s_count;
       int total = 0;
       for (int i = threadIdx.x; i < n; i += SH_WARPS * 32) {
-        const int a = idx[LR_MAX_TB + i];
+        const int a = list[i];
         out[2 + i] = a;
         total += p.first[a + 1] - p.first[a];
       }
@@ -122,7 +137,7 @@ __global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_ke
   }
   const int64_t row0 = (int64_t)blockIdx.x * (8 * NB);
   const int rows = (int)min((int64_t)(8 * NB), (int64_t)p.T - row0);
-  const int place = blockIdx.z % places, part = blockIdx.z / places;
+  const int z = blockIdx.z - lists, place = z / p.t_parts, part = z - place * p.t_parts, places = ((int)gridDim.z - lists) / p.t_parts;
   int count, only = -1;
   if constexpr (NB == 1) {                                    // every warp for itself: most blocks of threads find that there is nothing for them
     int a = lane < rows ? p.indx[row0 + lane] : -1;
@@ -135,12 +150,13 @@ __global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_ke
     only = __shfl_sync(0xFFFFFFFFu, a, __ffs(fresh) - 1);
     if (warp == 0 && lane < 8) s_idx[lane] = a;
   } else {
-    adapters_of(p, row0, rows, 8 * NB, s_idx, s_list, &s_count);
+    adapters_of<8 * NB>(p, row0, rows, s_idx, s_list, s_table, &s_count);
     count = s_count;
   }
   const int K8 = (p.K + 7) & ~7, blocks = (K8 + 31) >> 5, b0 = blocks * part / p.t_parts, b1 = blocks * (part + 1) / p.t_parts;
   for (int l = place; l < count; l += places) {
     const int a = NB == 1 ? only : s_list[l], f = p.first[a];
+    const float scale = p.scale[a];                           // (asked for here: behind the sums its trip to memory would be one more)
     if ((int)blockIdx.y >= p.first[a + 1] - f) continue;      // (uniform)
     const T16* ra = (const T16*)p.a + (int64_t)(f + blockIdx.y) * LR_PIECE * p.ld_a;
     float acc[NB][4];
@@ -177,7 +193,6 @@ __global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_ke
 #pragma unroll
     for (int n = 0; n < NB; ++n) *reinterpret_cast<float4*>(s_sum[warp][n][lane]) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
     __syncthreads();
-    const float scale = p.scale[a];
     for (int i = threadIdx.x; i < NB * 128; i += SH_WARPS * 32) {
       const int n = i >> 7, token = i >> 4, rank = i & 15;    // accumulator: rank rows, token columns
       const int ln = (rank & 7) * 4 + ((token & 7) >> 1), j = (rank >> 3) * 2 + (token & 1);
@@ -190,7 +205,6 @@ __global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_ke
     __syncthreads();
   }
 }
-static_assert(2 * LR_MAX_TB * sizeof(int) <= SH_WARPS * 32 * 4 * sizeof(float), "lists in place of the sums");
 
 // ---- pieces as MMA operands --------------------------------------------------------------------------------------
 // Operands of 16 k without swizzle: eight rows of 16 bytes are 128 bytes in a row, the two halves of k follow one another, then the next eight rows.
@@ -810,11 +824,13 @@ ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   s.nb = T <= 1024 ? 1 : 8;
   const int most = s.nb == 1 ? 8 : 4;                         // (a place without an adapter costs a block of threads all the same)
   s.places = n_adapters < most ? n_adapters : most;
-  // shares of k while the blocks that have something to do, a quarter of them say, are fewer than the SMs
+  // shares of k while the blocks that have something to do, a quarter of them say, are hardly more than the SMs
   const int64_t blocks = cdiv64(T, 8 * s.nb) * max_pieces * (s.nb == 1 && s.places > 2 ? s.places / 2 : 1);
   int parts = 1;
-  while (parts < LR_MAX_PARTS && blocks * parts <= moe_sm_count() && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
+  while (parts < LR_MAX_PARTS && blocks * parts <= moe_sm_count() * 3 / 2 && K / (32 * SH_WARPS) >= 2 * parts) parts *= 2;
   s.parts = parts;
+  // no more than some two and a half rounds of blocks (two per SM) for the sake of places, most of which find no adapter
+  while (s.nb > 1 && s.places > 1 && blocks * parts * s.places > 5 * moe_sm_count()) s.places = (s.places + 1) / 2;
   return s;
 }
 
@@ -928,9 +944,9 @@ int lr_allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
 template <typename K> int lr_allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) { return lr_allow_smem((const void*)kernel, bytes, done); }
 
 template <typename T16> int lr_shrink(const LoraParams& p, const ShrinkPlan& sp, cudaStream_t st) {
-  const dim3 grid((unsigned)cdiv64(p.T, 8 * sp.nb), (unsigned)(p.max_pieces + (p.list_tb > 0 ? 1 : 0)), (unsigned)(sp.places * sp.parts));
-  if (sp.nb == 1) MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 1>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
-  else MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 8>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p, sp.places));
+  const dim3 grid((unsigned)cdiv64(p.T, 8 * sp.nb), (unsigned)p.max_pieces, (unsigned)(sp.places * sp.parts + (p.list_tb > 0 ? 1 : 0)));
+  if (sp.nb == 1) MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 1>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p));
+  else MOE_CHECK_CUDA(launch_pdl(lora_shrink_kernel<T16, 8>, grid, dim3(SH_WARPS * 32), (size_t)0, st, p));
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
