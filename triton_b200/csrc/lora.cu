@@ -267,20 +267,23 @@ __device__ __forceinline__ bool cluster_fine(uint32_t at, int n) {
 // The shares of k of a cluster's CTAs meet, in their order: sums [token][128 outputs] at `at` in the shared memory of the CTAs step * r + base, r < S <=
 // MOST.  Tokens t0 .. t1 of the block for outputs n0 on; four outputs a thread, U of those and all shares on their way at a time (one share after the other
 // the sums of 300 tokens took 6 us).
+// (a thread's items there are a multiple of 32 apart, so its outputs are the same four: their biases are asked for before the CTAs wait for one another)
+__device__ __forceinline__ void sums_bias(const LoraParams& p, int n0, float (&bias)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + (threadIdx.x & 31) * 4 + j;
+    bias[j] = p.bias && n < p.N ? load_bias(p.bias, p.bias_dtype, n) : 0.0f;
+  }
+}
 template <typename T16, int MOST, int U>
-__device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, int S, uint32_t step, uint32_t base, int64_t row0, int t0, int t1, int n0) {
+__device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, int S, uint32_t step, uint32_t base, int64_t row0, int t0, int t1, int n0, const float (&bias)[4]) {
   const bool vec = p.N % 4 == 0 && p.ld_y % 4 == 0 && ((uintptr_t)p.y & 7u) == 0;
   uint32_t from[MOST];
 #pragma unroll
   for (int r = 0; r < MOST; ++r)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from[r]) : "r"(at), "r"(step * (uint32_t)min(r, S - 1) + base));
   for (int i0 = threadIdx.x; i0 < (t1 - t0) * 32; i0 += U * blockDim.x) {
-    float q[U][MOST][4], bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p.bias) {                                             // (a thread's items are a multiple of 32 apart: the same outputs)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n0 + (i0 & 31) * 4 + j < p.N) bias[j] = load_bias(p.bias, p.bias_dtype, n0 + (i0 & 31) * 4 + j);
-    }
+    float q[U][MOST][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = min(i0 + u * (int)blockDim.x, (t1 - t0) * 32 - 1);
@@ -532,10 +535,12 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     }
     tc_fence_before();
   }
+  float bias[4];
+  sums_bias(p, n0, bias);
   __syncthreads();
   if (S > 1) cluster_sync_all();
   const bool ok = cluster_fine(smem_u32(&s_abort), S);
-  if (ok) cluster_sums<T16, LS_MAX_SPLITS, 2>(p, sbase, S, 1u, 0u, row0, rows * rank / S, rows * (rank + 1) / S, n0);
+  if (ok) cluster_sums<T16, LS_MAX_SPLITS, 2>(p, sbase, S, 1u, 0u, row0, rows * rank / S, rows * (rank + 1) / S, n0, bias);
   if (S > 1) cluster_sync_all();                              // no CTA leaves while its sums are read
   if (warp == 1) {
     tc_fence_after();
@@ -767,16 +772,18 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
     if (!ok) __nanosleep(500000);
   }
   tc_fence_before();
+  const int sums_n0 = tile0 % pl.tiles_n * 256 + (int)half_id * LR_TILE_N;
+  float bias[4];
+  if (S > 1) sums_bias(p, sums_n0, bias);
   __syncthreads();
   cluster_sync_all();
   if (S > 1) {
     // ---- the splits' sums meet, in their order: each CTA takes a share of the tokens of its half of the outputs ----
     const bool ok = cluster_fine(smem_u32(&s_abort), 2 * S);
     if (ok && tile0 < tile1) {
-      const int block = tile0 / pl.tiles_n, n0 = (tile0 - block * pl.tiles_n) * 256 + (int)half_id * LR_TILE_N;
-      const int64_t row0 = (int64_t)block * TB;
+      const int64_t row0 = (int64_t)(tile0 / pl.tiles_n) * TB;
       const int rows = (int)min((int64_t)TB, (int64_t)p.T - row0);
-      cluster_sums<T16, LP_MAX_SPLITS, 4>(p, sbase, S, 2u, half_id, row0, rows * split / S, rows * (split + 1) / S, n0);
+      cluster_sums<T16, LP_MAX_SPLITS, 4>(p, sbase, S, 2u, half_id, row0, rows * split / S, rows * (split + 1) / S, sums_n0, bias);
     }
     cluster_sync_all();                                       // no CTA leaves while its sums are read
   }
