@@ -337,7 +337,8 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
   __shared__ __align__(8) uint64_t bars[2 * LS_MAX_STAGES + 1];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ int s_idx[LS_MAX_TB], s_first[LS_MAX_TB], s_from[LS_MAX_TB], s_count;
+  __shared__ __align__(16) int s_idx[LS_MAX_TB];
+  __shared__ int s_first[LS_MAX_TB], s_from[LS_MAX_TB], s_count;
   __shared__ unsigned long long s_mask[LS_MAX_TB];             // the tokens of an adapter
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int TB = pl.tb;
@@ -424,25 +425,40 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     }
     adapter_bar();
     // an adapter counts at its first token: its tokens and its pieces, the pieces numbered through
-    if (warp == 6) {
+    if (warp == 6) {                                          // a lane has tokens lane and lane + 32, side by side
+      uint32_t mask[2][2] = {{0u, 0u}, {0u, 0u}};
+      const int a[2] = {lane < TB ? s_idx[lane] : -1, lane + 32 < TB ? s_idx[lane + 32] : -1};
+#pragma unroll
+      for (int i = 0; i < LS_MAX_TB; i += 4) {
+        if (i >= TB) break;                                   // (a multiple of 16)
+        const int4 v = *reinterpret_cast<const int4*>(s_idx + i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          mask[h][i >> 5] |= (uint32_t)((v.x == a[h] ? 1 : 0) | (v.y == a[h] ? 2 : 0) | (v.z == a[h] ? 4 : 0) | (v.w == a[h] ? 8 : 0)) << (i & 31);
+      }
+      int f[2], np[2];
+      bool fresh[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        fresh[h] = a[h] >= 0 && (h == 0 ? (mask[0][0] & ((1u << lane) - 1u)) == 0 : mask[1][0] == 0 && (mask[1][1] & ((1u << lane) - 1u)) == 0);
+        f[h] = fresh[h] ? p.first[a[h]] : 0;
+        np[h] = fresh[h] ? p.first[a[h] + 1] : 0;
+      }
       int run = 0;
-      for (int t0 = 0; t0 < TB; t0 += 32) {
-        const int t = t0 + lane, a = t < TB ? s_idx[t] : -1;
-        unsigned long long mask = 0;
-        if (a >= 0)
-          for (int i = 0; i < TB; ++i) mask |= (unsigned long long)(s_idx[i] == a) << i;
-        const bool fresh = mask != 0 && __ffsll((long long)mask) - 1 == t;
-        const int f = fresh ? p.first[a] : 0, np = fresh ? p.first[a + 1] - f : 0;
-        int sum = np;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        np[h] -= f[h];
+        int sum = np[h];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int q = __shfl_up_sync(0xFFFFFFFFu, sum, o);
           if (lane >= o) sum += q;
         }
+        const int t = lane + 32 * h;
         if (t < TB) {
-          s_mask[t] = mask;
-          s_first[t] = f;
-          s_from[t] = run + sum - np;                         // (of tokens that are not the first of their adapter: no pieces)
+          s_mask[t] = a[h] >= 0 ? (unsigned long long)mask[h][1] << 32 | mask[h][0] : 0ull;
+          s_first[t] = f[h];
+          s_from[t] = run + sum - np[h];                      // (of tokens that are not the first of their adapter: no pieces)
         }
         run += __shfl_sync(0xFFFFFFFFu, sum, 31);
       }
