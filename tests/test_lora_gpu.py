@@ -108,6 +108,21 @@ def test_many_adapters(T):
 
 
 @gpu
+@pytest.mark.parametrize("T", [64, 512, 1100])
+@pytest.mark.parametrize("order", ["every", "turns", "back"])
+def test_order_of_the_adapters(T, order):
+    """as many adapters as tokens, one token each; three in turns; the last adapter's tokens first"""
+    L = {"every": T, "turns": 3, "back": 5}[order]
+    x, w, b, la, lb, scale = make(T, 64, 136, [1 + i % 17 for i in range(L)], torch.bfloat16, 11)
+    at = torch.arange(T, device="cuda")
+    indx = {"every": at * 37 % T, "turns": at % 3, "back": L - 1 - at * L // T}[order].to(torch.int32)
+    assert order != "every" or indx.unique().numel() == T
+    y = tb.matmul_lora(x, tb.prepare_projection_weight(w), b, tb.prepare_lora_adapters(la, lb, scale), indx)
+    tb.matmul_check_status()
+    check(y, *reference(x, w, b, la, lb, scale, indx))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T", [1, 40, 700])
 def test_without_adapters(T, dtype):

@@ -52,7 +52,7 @@ def reference(x, wg, bg, lw, full1, full2, k):
     def rounding(n):
         return (n / 32 + 64) * 2.0 ** -23
 
-    # a logit: a thread's 8 ceil(d / 2048) products one after the other, then 5 steps of a warp, 8 warps and the bias, half a step each
+    # a logit: at most 8 ceil(d / 2048) products one after the other, then 5 steps of a warp, the warps' sums in pairs and the bias, half a step each
     router_terms = 8 * -(-d // 2048) + 14
     b = torch.zeros(wg.shape[1], dtype=torch.float64, device=x.device) if bg is None else bg.double()
     logits, e_logit = X @ WG + b, router_terms * 2.0 ** -24 * (X.abs() @ WG.abs() + b.abs())
@@ -129,6 +129,19 @@ def test_token_counts(T, dtype):
 ])
 def test_shapes(T, E, k, d, ff):
     run_case(T, E, k, d, ff, seed=3)
+
+
+@gpu
+@pytest.mark.parametrize("T,E,k,d,ff", [(16, 64, 8, 1024, 96), (16, 8, 1, 2048, 1024), (11, 40, 3, 160, 1056)])
+def test_popular_experts(T, E, k, d, ff):
+    """some experts have one block of token columns and others two: the CTAs' shares differ"""
+    lw, full1, full2 = make_layer(E, d, ff, 5)
+    wg, bg = router(d, E, 5)
+    bg = bg + torch.linspace(0, 3, E, device="cuda").to(bg.dtype).flip(0)
+    x = torch.randn(T, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(12)).bfloat16()
+    y = tb.moe_layer_tokens(x, wg, bg, lw, k)
+    tb.matmul_check_status()
+    check(y, *reference(x, wg, bg, lw, full1, full2, k))
 
 
 @gpu

@@ -149,11 +149,15 @@ moe_tokens_router_kernel(const TX* x, int64_t ld_x, int T, int d, const __nv_bfl
   if (lane % (32 / TP) == 0) s_sum[warp][lane / (32 / TP)] = acc[0];
   __syncthreads();
   if (threadIdx.x < T) {
-    float v = 0.0f;
+    float v[WARPS];
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) v += s_sum[w][threadIdx.x];
-    if (bg) v += load_bias(bg, bg_dtype, e);
-    logits[threadIdx.x * E + e] = v;
+    for (int w = 0; w < WARPS; ++w) v[w] = s_sum[w][threadIdx.x];
+#pragma unroll
+    for (int n = WARPS / 2; n >= 1; n >>= 1)                  // (pairwise: four roundings)
+#pragma unroll
+      for (int w = 0; w < n; ++w) v[w] += v[w + n];
+    if (bg) v[0] += load_bias(bg, bg_dtype, e);
+    logits[threadIdx.x * E + e] = v[0];
   }
 }
 
