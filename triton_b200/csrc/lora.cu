@@ -465,12 +465,17 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
       if (lane == 0) s_count = run;
     }
     adapter_bar();
-    // every S-th piece is this CTA's, with each of its adapter's tokens
+    // Every S-th piece is this CTA's, with each of its adapter's tokens.  Few pieces go to all CTAs, and a piece's tokens by twos: 64 tokens of one
+    // adapter took 27.6 us with its one piece in one CTA, 17.4 this way.  (With up to 4 S pieces
+    // dealt out so, 16 tokens of an adapter each took 17.4 in place of 13.8: a look at each piece in every CTA.)
     const uint8_t* b = p.b + (int64_t)(n0 >> 3) * 256;
-    const int n_mine = s_count > rank ? (s_count - rank + S - 1) / S : 0;
+    const bool spread = s_count <= S;
+    const int from = spread ? 0 : rank, by = spread ? 1 : S, n_mine = s_count > from ? (s_count - from + by - 1) / by : 0;
+    unsigned long long twos = 0;                              // tokens 0, 1, 2 S, 2 S + 1, 4 S, ..
+    for (int t = 0; t < TB; t += 2 * S) twos |= 3ull << t;
     // -> the list place of this CTA's j-th piece, and which of that adapter's pieces it is
     auto find = [&](int j, int& l, int& i) {
-      const int g = rank + S * j;
+      const int g = from + by * j;
       int lo = 0, hi = TB;                                    // the last place that starts at or before g is the one with pieces
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -494,6 +499,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
         l = __shfl_sync(0xFFFFFFFFu, my_l, j & 31);
         i = __shfl_sync(0xFFFFFFFFu, my_i, j & 31);
         mask = s_mask[l] & mine_of;
+        if (spread) mask &= twos << (2 * ((rank + S - j % S) % S));
       }
       t = __ffsll((long long)mask) - 1;
       mask &= mask - 1;
@@ -844,7 +850,10 @@ int lr_map(const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows, 
 struct ShrinkPlan { int nb, places, parts; };
 ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   ShrinkPlan s;
-  s.nb = T <= 1024 ? 1 : 8;
+  // Eights read an adapter's rows more often, sixty-fours have fewer blocks for the adapters of single tokens.  K = 2880, N = 5120, 32 adapters of one piece, eights
+  // against sixty-fours, us of the whole operator: tokens in turns 512 65 : 98, 1024 95 : 136, 2048 179 : 259, 4096 290 : 450; in runs 512 33 : 34, 1024 44.6 : 46.1,
+  // 2048 73.7 : 75.3, 4096 115 : 109.  1200 tokens in runs, adapters of up to four pieces: 28.5 : 26.7.
+  s.nb = T <= 1024 || T * max_pieces <= 2048 ? 1 : 8;
   const int most = s.nb == 1 ? 8 : 4;                         // (a place without an adapter costs a block of threads all the same)
   s.places = n_adapters < most ? n_adapters : most;
   // shares of k while the blocks that have something to do, a quarter of them say, are hardly more than the SMs
@@ -936,7 +945,10 @@ PairPlan lr_pair_plan(int64_t T, int K, int N) {
   best.smem = bytes + 1024;
   return best;
 }
-// Up to 64 tokens weight rows by themselves fill the SMs (two CTAs each); beyond, a pair reads the tokens half as often.
+// Up to 64 tokens, decode's batches, weight rows by themselves fill the SMs (two CTAs each), and a token with an adapter of its own costs some fma; beyond,
+// a pair reads the tokens half as often, and a run of tokens of one adapter costs an MMA.  K = 2880, N = 5120, stream against pair, us: 32 adapters in
+// turns, 32 tokens 16.4 : 29.7, 64 20.5 : 30.2, 128 24.1 : 33.3, 256 40 : 35; one adapter per 64 tokens, 32 tokens 14.1 : 15.4, 64 17.4 : 16.4, 128 28.7 :
+// 18.4, 256 33 : 22.
 bool lr_many(int64_t T) { return T > 64; }
 
 size_t lr_t_bytes(const MoeLoraArgs& a, ShrinkPlan s) { return ((size_t)s.parts * (size_t)a.T * (size_t)a.max_pieces * LR_PIECE * 4 + 255) / 256 * 256; }
