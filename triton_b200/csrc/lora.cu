@@ -945,11 +945,11 @@ PairPlan lr_pair_plan(int64_t T, int K, int N) {
   best.smem = bytes + 1024;
   return best;
 }
-// Up to 64 tokens, decode's batches, weight rows by themselves fill the SMs (two CTAs each), and a token with an adapter of its own costs some fma; beyond,
+// Up to 128 tokens, decode's batches, weight rows by themselves fill the SMs (two CTAs each), and a token with an adapter of its own costs some fma; beyond,
 // a pair reads the tokens half as often, and a run of tokens of one adapter costs an MMA.  K = 2880, N = 5120, stream against pair, us: 32 adapters in
-// turns, 32 tokens 16.4 : 29.7, 64 20.5 : 30.2, 128 24.1 : 33.3, 256 40 : 35; one adapter per 64 tokens, 32 tokens 14.1 : 15.4, 64 17.4 : 16.4, 128 28.7 :
-// 18.4, 256 33 : 22.
-bool lr_many(int64_t T) { return T > 64; }
+// turns, 32 tokens 16.9 : 29.7, 64 21.0 : 30.2, 96 22.5 : 31.2, 128 25.1 : 33.3, 256 42.5 : 35.3; one adapter per 64 tokens, 32 tokens 14.3 : 15.4, 64 17.5 :
+// 16.4, 96 18.9 : 17.4, 128 21.0 : 18.4, 256 35.3 : 22.5.
+bool lr_many(int64_t T) { return T > 128; }
 
 size_t lr_t_bytes(const MoeLoraArgs& a, ShrinkPlan s) { return ((size_t)s.parts * (size_t)a.T * (size_t)a.max_pieces * LR_PIECE * 4 + 255) / 256 * 256; }
 size_t lr_list_bytes(const MoeLoraArgs& a) { return lr_many(a.T) ? (size_t)lr_pair_plan(a.T, a.K, a.N).blocks * LR_LIST * 4 : 0; }
