@@ -172,6 +172,18 @@ def test_layouts_of_the_inputs(T):
 
 @gpu
 @pytest.mark.parametrize("T", [10, 300])
+def test_broadcast_inputs(T):
+    x, w, b, la, lb, scale = make(T, 256, 200, [16, 24, 8], torch.bfloat16, 6)
+    indx = indices(T, 3, "random", 6)
+    adapters = tb.prepare_lora_adapters(la, lb, scale)
+    row, column, one = x[:1].expand(T, -1), w[:, :1].expand(-1, 200), indx[:1].expand(T)
+    got = tb.matmul_lora(row, column, b, adapters, indx)
+    assert torch.equal(got, tb.matmul_lora(row.clone(memory_format=torch.contiguous_format), tb.prepare_projection_weight(column.clone(memory_format=torch.contiguous_format)), b, adapters, indx))
+    assert torch.equal(tb.matmul_lora(x, w, b, adapters, one), tb.matmul_lora(x, w, b, adapters, one.clone(memory_format=torch.contiguous_format)))
+
+
+@gpu
+@pytest.mark.parametrize("T", [10, 300])
 def test_captured_replayed_and_side_by_side(T):
     cases = []
     for seed in (1, 2):

@@ -341,7 +341,7 @@ void same_device(const Tensor& x, const Tensor& t, const char* what) {
 // a matrix whose rows the kernels load 16 bytes at a time: as it is, or copied
 Tensor aligned_rows(const Tensor& t) {
   const int64_t per = 16 / t.element_size();
-  return t.stride(1) == 1 && (t.size(0) < 2 || t.stride(0) % per == 0) && (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+  return t.stride(1) == 1 && (t.size(0) < 2 || (t.stride(0) % per == 0 && t.stride(0) >= t.size(1))) && (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 // w1, w2: (values, scales, bias) in the default tiles; the work runs on x's device, on its current stream

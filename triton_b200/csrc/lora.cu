@@ -1047,6 +1047,7 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
   const MoeLoraArgs& a = *args;
   if (a.T == 0) return MOE_OK;
   MOE_CHECK_ARG(a.x && a.w_t && a.y, "moe_lora_matmul: NULL argument");
+  MOE_CHECK_ARG(a.ld_x >= a.K && a.ld_w >= a.K, "moe_lora_matmul: rows of x and W^T are K values apart at least");
   MOE_CHECK_ARG(a.ld_x % 8 == 0 && a.ld_w % 8 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w_t % 16 == 0,
                 "moe_lora_matmul: rows of x and W^T must be 16-byte aligned");
   const bool adapters = a.n_adapters > 0 && a.max_pieces > 0;

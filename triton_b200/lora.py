@@ -75,7 +75,7 @@ def prepare_projection_weight(w: torch.Tensor) -> torch.Tensor:
     if w.ndim != 2 or w.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("prepare_projection_weight: a [d_in, d_out] matrix of bf16 or fp16")
     K, N = w.shape
-    if (K < 2 or w.stride(0) == 1) and (N < 2 or w.stride(1) % 8 == 0) and w.data_ptr() % 16 == 0 and (N > 1 or K % 8 == 0):
+    if (K < 2 or w.stride(0) == 1) and (N < 2 or (w.stride(1) % 8 == 0 and w.stride(1) >= K)) and w.data_ptr() % 16 == 0 and (N > 1 or K % 8 == 0):
         return w
     out = torch.empty((N, -(-K // 8) * 8), dtype=w.dtype, device=w.device)[:, :K].t()
     out.copy_(w)
