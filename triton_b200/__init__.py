@@ -1,6 +1,6 @@
 """triton_b200: the MoE hot path of triton_kernels (routing, ragged grouped GEMM bf16 x MXFP4 with
 fused bias / SwiGLU / routing-weight epilogue, combine, MXFP4 quantise / dequantise, expert-parallel
-dispatch / combine) as hand-written CUDA for sm_100a behind a C ABI (include/moe_b200.h).
+dispatch / combine; a whole layer for a few tokens; a projection with low-rank adapters of many requests) as hand-written CUDA for sm_100a behind a C ABI (include/moe_b200.h).
 
 Importing the package does not need a GPU; calling an operator does, and needs libmoe_b200.so
 (``python -m triton_b200.build``).  There is no fallback path."""
