@@ -386,7 +386,7 @@ int moe_layer_tokens(const MoeTokensArgs* args, void* stream);
  * value [g][h][r][c] is B's rank 8 h + c at output 8 g + r, zero past N; finite (the product of a block of tokens multiplies other
  * adapters' B by zero).  x, w_t, a: 16-byte aligned rows, x's padded to 8 values (of any finite contents past K where adapters are given).
  * bias (fp32, fp16 or bf16) and, with n_adapters = 0, everything of the adapters may be NULL.  workspace: 256-byte aligned,
- * moe_lora_matmul_workspace_bytes(args) bytes of any contents; calls that may overlap need one each.  Two kernels (one without adapters);
+ * moe_lora_matmul_workspace_bytes(args) bytes of any contents (NULL where that is 0); calls that may overlap need one each.  Two kernels (one without adapters, or for one token and adapters of up to 16 ranks);
  * bounded waits (status codes 11xx). */
 typedef struct {
   const void* x; int dtype; int64_t ld_x; int64_t T; int K, N;

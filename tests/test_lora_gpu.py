@@ -90,6 +90,19 @@ def test_shapes(T, K, N, ranks, kind):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,N", [(8, 8), (77, 300), (1000, 129), (2880, 5120)])
+def test_one_token_of_small_ranks(K, N, dtype):
+    x, w, b, la, lb, scale = make(1, K, N, [16, 3, 9], dtype, 13)
+    pw, adapters = tb.prepare_projection_weight(w), tb.prepare_lora_adapters(la, lb, scale)
+    for a in (-1, 0, 1, 2, 3):
+        indx = torch.tensor([a], device="cuda", dtype=torch.int32)
+        y = tb.matmul_lora(x, pw, b, adapters, indx)
+        tb.matmul_check_status()
+        check(y, *reference(x, w, b, la, lb, scale, indx))
+
+
+@gpu
 @pytest.mark.parametrize("T", [3, 500])
 def test_high_rank(T):
     run_case(T, 256, 256, [1024, 200], kind="random", seed=5)

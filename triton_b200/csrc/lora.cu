@@ -9,10 +9,10 @@
 //  2. the product: W's tiles and x's through a ring by TMA, tcgen05.mma.kind::f16 into fp32 in tensor memory; then, into the same accumulator, one MMA per
 //     piece and term: B's tile times the tokens' t, zero for the tokens of other adapters, so that a block of tokens may hold any mixture.  t enters in two
 //     terms (hi + lo, 16 bits of it in bf16), so it costs the result nothing.
-// The second has two forms: lora_stream_kernel for few tokens, whose adapters' part runs on CUDA cores beside the product, and lora_pair_kernel for many, as
-// above.
-// Measured, K = 2880, N = 5120, shrink + product: 1 token 4.6 + 12 us (the weight at 2.5 TB/s: the launch, the first loads and the meeting of the shares of k are
-// two thirds), 64 tokens with an adapter each of 1 to 64 ranks 7 + 20 (55 MB), 300 tokens 6.4 + 23, 8192 tokens 18 + 213 (1134 TFLOP/s).  What bounds
+// The second has two forms: lora_stream_kernel for few tokens, whose adapters' part runs on CUDA cores beside the product (one token's first part too), and
+// lora_pair_kernel for many, as above.
+// Measured, K = 2880, N = 5120, shrink + product: 1 token 9.3 us of one launch (29.7 MB at 3.2 TB/s; its start, the first loads and the meeting of the shares of
+// k are half), 64 tokens with an adapter each of 1 to 64 ranks 7 + 20 (55 MB), 300 tokens 6.4 + 23, 8192 tokens 18 + 213 (1134 TFLOP/s).  What bounds
 // the last: a CTA takes in 48 KB for 1024 cycles of MMA, and an SM some 32 B a cycle.
 #include "gemm_pair_common.cuh"
 #include <cuda_fp16.h>
@@ -325,7 +325,7 @@ __device__ __forceinline__ void cluster_sums(const LoraParams& p, uint32_t at, i
 constexpr int LS_THREADS = 320;                // warp 0 producer, 1 MMA, 2-9 adapters and then epilogue
 constexpr int LS_MAX_STAGES = 8, LS_MAX_TB = 64, LS_MAX_SPLITS = 6;
 
-struct StreamPlan { int tb, splits, stages, smem; };           // tokens of a block, cluster, ring of k steps, bytes
+struct StreamPlan { int tb, splits, stages, smem, direct; };   // tokens of a block, cluster, ring of k steps, bytes, x A made here
 
 __device__ __forceinline__ void adapter_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
@@ -343,6 +343,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
   __shared__ __align__(16) int s_idx[LS_MAX_TB];
   __shared__ int s_first[LS_MAX_TB], s_from[LS_MAX_TB], s_count;
   __shared__ unsigned long long s_mask[LS_MAX_TB];             // the tokens of an adapter
+  __shared__ float s_t[LR_PIECE];
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int TB = pl.tb;
   const uint32_t X_BYTES = (uint32_t)TB * 128u, stage_bytes = SUBTILE_BYTES + X_BYTES;
@@ -472,8 +473,8 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
     // adapter took 27.6 us with its one piece in one CTA, 17.4 this way.  (With up to 4 S pieces
     // dealt out so, 16 tokens of an adapter each took 17.4 in place of 13.8: a look at each piece in every CTA.)
     const uint8_t* b = p.b + (int64_t)(n0 >> 3) * 256;
-    const bool spread = s_count <= S;
-    const int from = spread ? 0 : rank, by = spread ? 1 : S, n_mine = s_count > from ? (s_count - from + by - 1) / by : 0;
+    const bool spread = s_count <= S, all = spread || pl.direct;
+    const int from = all ? 0 : rank, by = all ? 1 : S, n_mine = s_count > from ? (s_count - from + by - 1) / by : 0;
     unsigned long long twos = 0;                              // tokens 0, 1, 2 S, 2 S + 1, 4 S, ..
     for (int t = 0; t < TB; t += 2 * S) twos |= 3ull << t;
     // -> the list place of this CTA's j-th piece, and which of that adapter's pieces it is
@@ -502,13 +503,40 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
         l = __shfl_sync(0xFFFFFFFFu, my_l, j & 31);
         i = __shfl_sync(0xFFFFFFFFu, my_i, j & 31);
         mask = s_mask[l] & mine_of;
-        if (spread) mask &= twos << (2 * ((rank + S - j % S) % S));
+        if (spread && !pl.direct) mask &= twos << (2 * ((rank + S - j % S) % S));
       }
       t = __ffsll((long long)mask) - 1;
       mask &= mask - 1;
       return true;
     };
-    const float* ranks = p.t + row0 * p.ld_t + (lane & 15);   // a lane holds one of the sixteen ranks of a token
+    if (pl.direct) {
+      // x A over this CTA's share of k, two ranks a warp: as it is linear, B takes the share like the whole, and the shares of y meet as they do anyway
+      if (s_count > 0) {
+        const int k1 = min(kt1 * BLOCK_K, (p.K + 7) & ~7), r = (warp - 2) * 2;
+        const T16 *a = (const T16*)p.a + ((int64_t)s_first[0] * LR_PIECE + r) * p.ld_a, *x = (const T16*)p.x;
+        const float scale = p.scale[s_idx[0]];
+        float v[2] = {0.0f, 0.0f};
+#pragma unroll 2
+        for (int k = kt0 * BLOCK_K + lane * 8; k < k1; k += 256) {
+          const uint4 xv = *reinterpret_cast<const uint4*>(x + k), a0 = *reinterpret_cast<const uint4*>(a + k), a1 = *reinterpret_cast<const uint4*>(a + p.ld_a + k);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float f = to_f32<T16>(reinterpret_cast<const T16*>(&xv)[j]);
+            v[0] = fmaf(f, to_f32<T16>(reinterpret_cast<const T16*>(&a0)[j]), v[0]);
+            v[1] = fmaf(f, to_f32<T16>(reinterpret_cast<const T16*>(&a1)[j]), v[1]);
+          }
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+          v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+          v[1] += __shfl_xor_sync(0xFFFFFFFFu, v[1], o);
+        }
+        if (lane < 2) s_t[r + lane] = (lane ? v[1] : v[0]) * scale;
+      }
+      adapter_bar();
+    }
+    const float* ranks = (pl.direct ? s_t : p.t + row0 * p.ld_t) + (lane & 15);      // a lane holds one of the sixteen ranks of a token
+    const int parts = pl.direct ? 1 : p.t_parts;
     bool more = advance();
     // four pairs on their way: as one is taken on, the next takes its place
     constexpr int U = 4;
@@ -524,7 +552,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
       at[u] = t;
       rest[u] = t * (int)p.ld_t + i * LR_PIECE;
 #pragma unroll
-      for (int q = 0; q < LR_MAX_PARTS; ++q) r[u][q] = q < p.t_parts ? ranks[q * p.t_part_stride + rest[u]] : 0.0f;
+      for (int q = 0; q < LR_MAX_PARTS; ++q) r[u][q] = q < parts ? ranks[q * p.t_part_stride + rest[u]] : 0.0f;
       more = advance();
     };
 #pragma unroll
@@ -869,8 +897,13 @@ ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   return s;
 }
 
-StreamPlan lr_stream_plan(int64_t T, int K, int N) {
+// A token's x A within the product's kernel: saves a launch, and costs every CTA its share of A's rows, some 1 us a token and piece.  K = 2880, N = 5120: one
+// token and piece 10.2 us in place of 11.5, two 12.0 and 11.8, four 14.3 and 12.5, eight 19.0 and 12.5.
+bool lr_direct(int64_t T, int max_pieces) { return T * max_pieces <= 1; }
+
+StreamPlan lr_stream_plan(int64_t T, int K, int N, int max_pieces) {
   StreamPlan pl;
+  pl.direct = max_pieces > 0 && lr_direct(T, max_pieces);
   pl.tb = T >= LS_MAX_TB ? LS_MAX_TB : (int)cdiv64(T, 16) * 16;
   const int64_t tiles = cdiv64(N, LR_TILE_N) * cdiv64(T, pl.tb), KT = cdiv64(K, BLOCK_K);
   const int stage = SUBTILE_BYTES + pl.tb * 128, sums = pl.tb * LR_TILE_N * 4;
@@ -991,7 +1024,7 @@ template <typename T16> int lr_shrink(const LoraParams& p, const ShrinkPlan& sp,
 
 template <typename T16> int lr_stream(const LoraParams& p, const MoeLoraArgs& a, cudaStream_t st) {
   const bool f16 = std::is_same<T16, __half>::value;
-  const StreamPlan pl = lr_stream_plan(p.T, p.K, p.N);
+  const StreamPlan pl = lr_stream_plan(p.T, p.K, p.N, p.max_pieces);
   CUtensorMap w_map, x_map;
   if (int rc = lr_map(a.w_t, a.N, a.K, a.ld_w, LR_TILE_N, f16, &w_map)) return rc;
   if (int rc = lr_map(a.x, a.T, a.K, a.ld_x, pl.tb, f16, &x_map)) return rc;
@@ -1041,7 +1074,7 @@ template <typename T16> int lr_pair(const LoraParams& p, const MoeLoraArgs& a, c
 }  // namespace
 
 extern "C" __attribute__((visibility("default"))) size_t moe_lora_matmul_workspace_bytes(const MoeLoraArgs* a) {
-  if (lr_check(a) != MOE_OK || a->n_adapters == 0) return 0;
+  if (lr_check(a) != MOE_OK || a->n_adapters == 0 || lr_direct(a->T, a->max_pieces)) return 0;
   return lr_t_bytes(*a, lr_shrink_plan(a->T, a->K, a->max_pieces, a->n_adapters)) + lr_list_bytes(*a);
 }
 
@@ -1053,7 +1086,7 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
   MOE_CHECK_ARG(a.ld_x >= a.K && a.ld_w >= a.K, "moe_lora_matmul: rows of x and W^T are K values apart at least");
   MOE_CHECK_ARG(a.ld_x % 8 == 0 && a.ld_w % 8 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w_t % 16 == 0,
                 "moe_lora_matmul: rows of x and W^T must be 16-byte aligned");
-  const bool adapters = a.n_adapters > 0 && a.max_pieces > 0;
+  const bool adapters = a.n_adapters > 0 && a.max_pieces > 0, direct = adapters && lr_direct(a.T, a.max_pieces);
   ShrinkPlan sp = {1, 1, 1};
   if (adapters) {
     MOE_CHECK_ARG(a.a && a.b && a.first && a.scale && a.indx, "moe_lora_matmul: NULL argument of the adapters");
@@ -1061,8 +1094,8 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
                   "moe_lora_matmul: adapters must be 16-byte aligned, their rows padded to 8 values");
     MOE_CHECK_ARG(a.ld_x >= (a.K + 7) / 8 * 8, "moe_lora_matmul: rows of x must be padded to 8 values");
     sp = lr_shrink_plan(a.T, a.K, a.max_pieces, a.n_adapters);
-    const size_t need = lr_t_bytes(a, sp) + lr_list_bytes(a);
-    MOE_CHECK_ARG(a.workspace && (uintptr_t)a.workspace % 256 == 0 && a.workspace_bytes >= need,
+    const size_t need = direct ? 0 : lr_t_bytes(a, sp) + lr_list_bytes(a);
+    MOE_CHECK_ARG(need == 0 || (a.workspace && (uintptr_t)a.workspace % 256 == 0 && a.workspace_bytes >= need),
                   "moe_lora_matmul: needs a 256-byte aligned workspace of %zu bytes", need);
   }
   cudaStream_t st = (cudaStream_t)stream;
@@ -1081,7 +1114,7 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
     p.list = (int32_t*)((uint8_t*)a.workspace + lr_t_bytes(a, sp));
     p.list_tb = pl.tb;
   }
-  if (adapters)
+  if (adapters && !direct)
     if (int rc = a.dtype == MOE_F16 ? lr_shrink<__half>(p, sp, st) : lr_shrink<__nv_bfloat16>(p, sp, st)) return rc;
   if (many) return a.dtype == MOE_F16 ? lr_pair<__half>(p, a, pl, st) : lr_pair<__nv_bfloat16>(p, a, pl, st);
   return a.dtype == MOE_F16 ? lr_stream<__half>(p, a, st) : lr_stream<__nv_bfloat16>(p, a, st);

@@ -1,7 +1,7 @@
 """A dense projection that all requests share, with each request's own low-rank adapter beside it.
 
 The reference's `matmul` multiplies the rows of a ragged batch by their group's matrix (matmul.py:245-766); serving fine-tuned models puts one shared
-matrix under all rows and a small product of two thin matrices, another per request, on top.  `matmul_lora` does both in two kernels."""
+matrix under all rows and a small product of two thin matrices, another per request, on top.  `matmul_lora` does both in two kernels (one for a single token's adapter of up to 16 ranks)."""
 import itertools
 from dataclasses import dataclass
 from typing import Sequence
