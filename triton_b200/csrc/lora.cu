@@ -882,9 +882,9 @@ struct ShrinkPlan { int nb, places, parts; };
 ShrinkPlan lr_shrink_plan(int64_t T, int K, int max_pieces, int n_adapters) {
   ShrinkPlan s;
   // Eights read an adapter's rows more often, sixty-fours have fewer blocks for the adapters of single tokens.  K = 2880, N = 5120, 32 adapters of one piece, eights
-  // against sixty-fours, us of the whole operator: tokens in turns 512 65 : 98, 1024 95 : 136, 2048 179 : 259, 4096 290 : 450; in runs 512 33 : 34, 1024 44.6 : 46.1,
-  // 2048 73.7 : 75.3, 4096 115 : 109.  1200 tokens in runs, adapters of up to four pieces: 28.5 : 26.7.
-  s.nb = T <= 1024 || T * max_pieces <= 2048 ? 1 : 8;
+  // against sixty-fours, us of the whole operator: tokens in turns 512 65 : 98, 1024 95 : 136, 2048 179 : 259, 3000 205 : 345, 4096 290 : 440; in runs 512 33 : 34, 1024
+  // 44.6 : 46.1, 2048 73.7 : 75.3, 3000 93.7 : 96.3, 4096 115 : 109.  1200 tokens in runs, adapters of up to four pieces: 28.5 : 26.7.
+  s.nb = T <= 1024 || T * max_pieces <= 3500 ? 1 : 8;
   const int most = s.nb == 1 ? 8 : 4;                         // (a place without an adapter costs a block of threads all the same)
   s.places = n_adapters < most ? n_adapters : most;
   // shares of k while the blocks that have something to do, a quarter of them say, are hardly more than the SMs
