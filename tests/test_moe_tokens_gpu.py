@@ -333,3 +333,64 @@ def test_refusals_of_the_c_entry_point():
     assert lib.moe_layer_tokens_workspace_bytes(None) == 0
     blank = (ctypes.c_uint8 * 512)()                           # all sizes zero
     assert lib.moe_layer_tokens(ctypes.addressof(blank), None) == 1 and b"positive" in lib.moe_last_error()
+
+
+def layer_of_differences(E, d, ff, seed):
+    """W1 = 0, so hidden value i is SwiGLU of its biases whatever the token; output o is h_i - h_j of two neighbours by size.  -> (MoeLayerWeights,
+    h [E, ff] in 64 bits, i [d], j [d])"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def laid_out(q, s):
+        return (tb.convert_layout(tb.wrap_torch_tensor(q.transpose(1, 2), dtype=tb.FP4), make_default_matmul_mxfp4_w_layout(mx_axis=-2)),
+                tb.convert_layout(tb.wrap_torch_tensor(s.transpose(1, 2)), make_default_matmul_mxfp4_w_scale_layout(mx_axis=-2)))
+
+    b1 = torch.empty(E, 2 * ff, device="cuda")
+    b1[:, 0::2] = torch.rand(E, ff, device="cuda", generator=g).sort(1).values * 0.02 + 1.0
+    b1[:, 1::2] = 0.25
+    gate, lin = b1[:, 0::2].double(), b1[:, 1::2].double()
+    h = gate * torch.sigmoid(1.702 * gate) * (lin + 1)
+    i = torch.randint(0, ff - 1, (d,), device="cuda", generator=g)
+    codes = torch.zeros(E, d, ff, dtype=torch.uint8, device="cuda")
+    codes.scatter_(2, i.view(1, d, 1).expand(E, -1, -1), 2)                    # 1.0
+    codes.scatter_(2, (i + 1).view(1, d, 1).expand(E, -1, -1), 2 | 8)          # -1.0
+    q1, s1 = torch.zeros(E, 2 * ff, d // 2, dtype=torch.uint8, device="cuda"), torch.full((E, 2 * ff, d // 32), 127, dtype=torch.uint8, device="cuda")
+    q2, s2 = codes[..., 0::2] | codes[..., 1::2] << 4, torch.full((E, d, ff // 32), 127, dtype=torch.uint8, device="cuda")
+    lw = MoeLayerWeights(*laid_out(q1, s1), b1, *laid_out(q2, s2), torch.zeros(E, d, device="cuda"))
+    return lw, h, i, i + 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (4, 1, 1), (5, 1, 1), (8, 1, 1), (8, 2, 2), (9, 1, 1), (16, 1, 1), (16, 3, 3), (13, 6, 2)])
+def test_hidden_rows_keep_their_bits_however_many_tokens_an_expert_has(T, E, k, dtype):
+    """A hidden value is good to 2^-20 of itself (the exponential and the division), its two terms to 2^-22 and each of the sum's few roundings to 2^-23: less than
+    2^-19 of the two values together, per expert; the gates sum to one within 2^-20 and weigh differences of some 2^-9; the result's own half step."""
+    d, ff = 96, 160
+    lw, h, i, j = layer_of_differences(E, d, ff, 3)
+    wg, bg = router(d, E, 3)
+    x = torch.randn(T, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(dtype)
+    y = tb.moe_layer_tokens(x, wg, bg, lw, k).double()
+    tb.matmul_check_status()
+    logits = x.double() @ wg.double() + bg.double()
+    vals, indx = torch.sort(logits, dim=1, descending=True, stable=True)
+    gates = torch.softmax(vals[:, :k], 1)
+    ref = torch.einsum("tk,tkd->td", gates, (h[:, i] - h[:, j])[indx[:, :k]])
+    e_gates = 2.0 ** -18 * (h[:, i] - h[:, j]).abs().amax(0)          # (logits of some ten roundings of values below 8: 2^-18)
+    bound = 2.0 ** -19 * (h[:, i] + h[:, j]).amax(0) + e_gates
+    bound = bound + (ref.abs() + bound) * torch.finfo(dtype).eps / 2
+    worst = ((y - ref).abs() / bound).max().item()
+    assert worst <= 1.0, f"{worst} of the bound"
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k,d,ff", [
+    (16, 16, 16, 512, 1056),        # every expert has all tokens: two entries of fc2 each, 256 picks
+    (8, 8, 8, 1440, 2880),          # fc2 in three stages, cut between CTAs
+    (8, 3, 3, 64, 8192),
+    (8, 3, 2, 8192, 64),
+    (12, 4, 2, 2880, 1024),         # some experts in two entries, others in one
+    (5, 2, 1, 736, 1440),
+])
+def test_experts_of_most_tokens(T, E, k, d, ff, dtype):
+    run_case(T, E, k, d, ff, dtype, seed=17)

@@ -20,8 +20,8 @@
 // Arithmetic: a code becomes fp16 exactly, tokens are fp16 scaled by their row's largest finite element, which is put in [2^13, 2^14):
 // elements down to 2^-30 of it keep all of bf16's bits.  mma.sync m16n8k16 sums one scale group of 32 k in fp32, which
 // is multiplied by the group's scale and added up in fp32.  The legacy tensor path is far more than 16 tokens need, and its fragments come straight
-// from the packed words.  SwiGLU outputs stay fp32 in the workspace; as operand they are fp16 of the row's scale, 2^-12 of a value off, in two terms
-// (2^-23) where the expert has at most half as many tokens as there are columns.
+// from the packed words.  SwiGLU outputs stay fp32 in the workspace; as operand they are two fp16 terms of the row's scale, 2^-23 of a value off (2^-38 of
+// the row's largest where it is that small).
 #include "gemm_tc_common.cuh"
 #include "topk_select.cuh"
 #include <cuda_fp16.h>
@@ -266,16 +266,17 @@ struct TokensShared {                   // beside ring, staged tokens and partia
   uint64_t full[MT_MAX_STAGES], empty[MT_MAX_STAGES];
   uint64_t sums[2], taken[2];           // a buffer of sums is complete, has been read
   int abort;
-  int n_active;
-  int act[MT_MAX_EXPERTS];              // active experts in ascending order
-  uint16_t rank[MT_MAX_EXPERTS];        // place of an expert in that list
-  uint32_t ahead[MT_MAX_EXPERTS + 1];   // by that place: time of a step of fc1 in all experts ahead (low half) and of fc2 (high half), see step_time
+  int n_active, n_entries;
+  uint8_t act[MT_MAX_EXPERTS];          // active experts in ascending order
+  uint8_t from[MT_MAX_EXPERTS];         // an expert's first entry of fc2
+  uint16_t entries[MT_MAX_EXPERTS];     // expert and (from bit 8 on) part of its tokens, see Entry; each has a token's pick, so there are at most 256
+  uint16_t ahead1[MT_MAX_EXPERTS + 1], ahead2[MT_MAX_EXPERTS + 1];     // time of a step of fc1 in all active experts ahead, of fc2 in all entries, see step_time
   alignas(16) uint32_t tokens[MT_MAX_EXPERTS];     // its tokens, a bit each
   uint8_t slot[MT_MAX_EXPERTS][MT_MAX_TOKENS];     // which pick of its tokens it is
   uint8_t who[MT_MAX_EXPERTS][MT_MAX_TOKENS];      // its tokens one behind the other
   uint8_t sel[MT_MAX_TOKENS][MT_MAX_K];
   float gate[MT_MAX_TOKENS][MT_MAX_K];
-  float undo1[MT_MAX_TOKENS];           // what the sums over staged rows are short of: of fc1's tokens, of fc2's last four experts
+  float undo1[MT_MAX_TOKENS];           // what the sums over staged rows are short of: of fc1's tokens, of fc2's last four entries
   float undo2[4][MT_MAX_TOKENS];
 };
 
@@ -344,14 +345,19 @@ __device__ __forceinline__ void stage_x(const TokensParams& p, TokensShared& s, 
   }
   if (lane == 0) s.undo1[t] = pow2(ex - 13);
 }
-// whether an expert's rows are staged in two terms
-__device__ __forceinline__ bool two_terms(int n, int nblk) { return 2 * n <= 8 * nblk; }
+// fc2 has every hidden row in two columns, a term each.  An expert with more tokens than half of the columns is two entries of fc2: the weights of the second are
+// read once more, mostly from L2 (with one term for the tokens of such experts a token's result hung on how many others had picked its expert, 2^-12
+// of a hidden value in place of 2^-23).
+struct Entry { int e, r0, n; };         // expert, first of its tokens, how many of them
+template <int NBLK> __device__ __forceinline__ Entry entry_of(const TokensShared& s, int place) {
+  const int v = s.entries[place], e = v & 255, r0 = (v >> 8) * 4 * NBLK;
+  return {e, r0, min(__popc(s.tokens[e]) - r0, 4 * NBLK)};
+}
 
-// An expert's hidden rows as the columns of fc2 (n of them), behind one another, their second terms behind the first: a warp takes 256 k of a row,
+// An entry's hidden rows as the columns of fc2, behind one another, their second terms behind the first: a warp takes 256 k of a row,
 // two at a time
-__device__ __forceinline__ void stage_h(const TokensParams& p, TokensShared& s, int nblk, uint32_t toks, int e, int n, int KT2, int place, int warp) {
-  const int lane = threadIdx.x & 31;
-  const bool two = two_terms(n, nblk);
+__device__ __forceinline__ void stage_h(const TokensParams& p, TokensShared& s, int nblk, uint32_t toks, const Entry& en, int KT2, int place, int warp) {
+  const int lane = threadIdx.x & 31, n = en.n, e = en.e;
   const int chunks = (KT2 + 1) >> 1, total = n * chunks;
   for (int i0 = warp; i0 < total; i0 += 2 * MT_WARPS) {   // 256 k of a row by a warp, two at a time
     float4 raw[2][2];
@@ -362,7 +368,7 @@ __device__ __forceinline__ void stage_h(const TokensParams& p, TokensShared& s, 
       raw[x][0] = raw[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       mx[x] = 0.0f;
       if (i < total) {
-        const int t = s.who[e][r], entry = t * p.k + s.slot[e][t];
+        const int t = s.who[e][en.r0 + r], entry = t * p.k + s.slot[e][t];
         mx[x] = __uint_as_float(__ldcg(p.hmax + entry));
         if (k8 * 8 < p.ff) {
           const float4* src = reinterpret_cast<const float4*>(p.h + (int64_t)entry * p.ff + k8 * 8);
@@ -384,36 +390,34 @@ __device__ __forceinline__ void stage_h(const TokensParams& p, TokensShared& s, 
         w[j] = isfinite(left) ? left : 0.0f;
       }
       sts128(tok_at(toks, nblk, r, k8), pack8(v));
-      if (two) sts128(tok_at(toks, nblk, n + r, k8), pack8(w));
+      sts128(tok_at(toks, nblk, n + r, k8), pack8(w));
       if (k8 == 0) s.undo2[place][r] = pow2(ex - 13);
     }
   }
 }
 
-// What a stage takes the tensor-core loop, relative to others: the columns' second block of eight costs half as much as everything else.  (Dealt out
+// What a stage of `columns` columns takes the tensor-core loop, relative to others: the second block of eight costs half as much as everything else.  (Dealt out
 // evenly, 13 tokens of 64 experts, k = 8, took 71 us in place of 66: the last CTA came 8 us behind the mean.)
-__device__ __forceinline__ uint32_t step_time(int n, int nblk) {
-  return nblk == 1 ? 0x10001u : (n > 8 ? 3u : 2u) + ((two_terms(n, nblk) ? 2 * n : n) > 8 ? 0x30000u : 0x20000u);
-}
-// Steps of a product, `per` an expert, are dealt out to CTAs by that time.  The CTA of a step: where the time ahead of it falls.
-template <int NBLK, int SHIFT>
-__device__ __forceinline__ int cta_of(const TokensShared& s, int step, int place, int per, int total, int G) {
+__device__ __forceinline__ uint32_t step_time(int columns, int nblk) { return nblk == 1 ? 1u : columns > 8 ? 3u : 2u; }
+// Steps of a product, `per` an expert or entry, are dealt out to CTAs by that time.  The CTA of a step: where the time ahead of it falls.
+template <int NBLK>
+__device__ __forceinline__ int cta_of(const uint16_t* aheads, int step, int place, int per, int total, int G) {
   if (NBLK == 1) return step * G / total;
-  const int ahead = (s.ahead[place] >> SHIFT) & 0xFFFF, each = ((s.ahead[place + 1] >> SHIFT) & 0xFFFF) - ahead;
+  const int ahead = aheads[place], each = aheads[place + 1] - ahead;
   return (ahead * per + (step - place * per) * each) * G / total;
 }
 // The first step of CTA c, by a warp: cta_of is c or more from there on
-template <int NBLK, int SHIFT>
-__device__ __forceinline__ int first_step(const TokensShared& s, int c, int per, int total, int G, const Div& by_ctas) {
+template <int NBLK>
+__device__ __forceinline__ int first_step(const uint16_t* aheads, int places, int c, int per, int total, int G, const Div& by_ctas) {
   const int time = (total * c + G - 1) / by_ctas;
   if (NBLK == 1) return time;
-  int place = -1;                       // the last expert that begins at that time or before
+  int place = -1;                       // the last one that begins at that time or before
 #pragma unroll
   for (int i = 0; i < MT_MAX_EXPERTS / 32; ++i) {
     const int a = i * 32 + (threadIdx.x & 31);
-    if (i * 32 < s.n_active) place += __popc(__ballot_sync(0xFFFFFFFFu, a < s.n_active && (int)((s.ahead[a] >> SHIFT) & 0xFFFF) * per <= time));
+    if (i * 32 < places) place += __popc(__ballot_sync(0xFFFFFFFFu, a < places && aheads[a] * per <= time));
   }
-  const int ahead = (s.ahead[place] >> SHIFT) & 0xFFFF, each = ((s.ahead[place + 1] >> SHIFT) & 0xFFFF) - ahead;
+  const int ahead = aheads[place], each = aheads[place + 1] - ahead;
   return place * per + (time - ahead * per + each - 1) / each;
 }
 
@@ -453,14 +457,15 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     if (warp < MT_WARPS / 2)
       for (int t = warp; t < p.T; t += MT_WARPS / 2) select_token(p, s, t, lane);
     bar_sync(3, OTHERS);
-    if (warp == MT_WARPS) {             // the list of active experts, eight a lane
+    if (warp == MT_WARPS) {             // the lists of active experts and of fc2's entries, eight experts a lane; fc1's figures in low halves, fc2's in high ones
+      constexpr int HALF = 4 * NBLK;    // tokens of an entry
       uint32_t takes[8], on = 0, time = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int n = __popc(s.tokens[lane * 8 + i]);
-        takes[i] = n ? step_time(n, NBLK) : 0u;
+        takes[i] = n ? step_time(n, NBLK) | (step_time(2 * min(n, HALF), NBLK) + (n > HALF ? step_time(2 * (n - HALF), NBLK) : 0u)) << 16 : 0u;
         time += takes[i];
-        on += n ? 1u : 0u;
+        on += n ? (n > HALF ? 0x20001u : 0x10001u) : 0u;
       }
       uint32_t at = on, ahead = time;
 #pragma unroll
@@ -468,16 +473,31 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         const uint32_t q = __shfl_up_sync(0xFFFFFFFFu, at, o), w = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
         if (lane >= o) { at += q; ahead += w; }
       }
-      if (lane == 31) { s.n_active = (int)at; s.ahead[at] = ahead; }
+      if (lane == 31) {
+        s.n_active = (int)(at & 0xFFFFu);
+        s.n_entries = (int)(at >> 16);
+        s.ahead1[at & 0xFFFFu] = (uint16_t)ahead;
+        s.ahead2[at >> 16] = (uint16_t)(ahead >> 16);
+      }
       at -= on;
       ahead -= time;
+      int a1 = (int)(at & 0xFFFFu), a2 = (int)(at >> 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (takes[i]) {
-          s.act[at] = lane * 8 + i;
-          s.rank[lane * 8 + i] = (uint16_t)at;
-          s.ahead[at] = ahead;
-          ++at;
+          const int e = lane * 8 + i;
+          s.act[a1] = (uint8_t)e;
+          s.ahead1[a1] = (uint16_t)ahead;
+          ++a1;
+          s.from[e] = (uint8_t)a2;
+          s.entries[a2] = (uint16_t)e;
+          s.ahead2[a2] = (uint16_t)(ahead >> 16);
+          ++a2;
+          if (__popc(s.tokens[e]) > HALF) {
+            s.entries[a2] = (uint16_t)(e | 256);
+            s.ahead2[a2] = (uint16_t)((ahead >> 16) + step_time(2 * HALF, NBLK));
+            ++a2;
+          }
           ahead += takes[i];
         }
     } else if (threadIdx.x < p.T * p.k) {
@@ -489,14 +509,14 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   }
   if (warp < MT_WARPS) bar_sync(1, MT_CONSUMERS);
 
-  const int A = s.n_active, G = gridDim.x, c = blockIdx.x;
+  const int A = s.n_active, A2 = s.n_entries, G = gridDim.x, c = blockIdx.x;
   const int KT1 = (p.d + 127) >> 7, KT2 = (p.ff + 127) >> 7, KS1 = (KT1 + MT_STAGE_KT - 1) / MT_STAGE_KT, KS2 = (KT2 + MT_STAGE_KT - 1) / MT_STAGE_KT;
   const int NB1 = 2 * p.ff / MT_UNIT, NB2 = p.d / MT_UNIT, NT1 = (2 * p.ff + 127) >> 7, NT2 = (p.d + 127) >> 7;
   const int U1 = A * NB1;
-  const int time1 = (int)(s.ahead[A] & 0xFFFF) * NB1, time2 = (int)(s.ahead[A] >> 16) * NB2 * KS2;      // (times the CTAs below 2^26: the widths' limits)
-  const int u_begin = first_step<NBLK, 0>(s, c, NB1, time1, G, p.by_ctas), u_end = c + 1 == G ? U1 : first_step<NBLK, 0>(s, c + 1, NB1, time1, G, p.by_ctas);
-  const int s_begin = first_step<NBLK, 16>(s, c, NB2 * KS2, time2, G, p.by_ctas);
-  const int s_end = c + 1 == G ? A * NB2 * KS2 : first_step<NBLK, 16>(s, c + 1, NB2 * KS2, time2, G, p.by_ctas);
+  const int time1 = s.ahead1[A] * NB1, time2 = s.ahead2[A2] * NB2 * KS2;      // (times the CTAs below 2^26: the widths' limits)
+  const int u_begin = first_step<NBLK>(s.ahead1, A, c, NB1, time1, G, p.by_ctas), u_end = c + 1 == G ? U1 : first_step<NBLK>(s.ahead1, A, c + 1, NB1, time1, G, p.by_ctas);
+  const int s_begin = first_step<NBLK>(s.ahead2, A2, c, NB2 * KS2, time2, G, p.by_ctas);
+  const int s_end = c + 1 == G ? A2 * NB2 * KS2 : first_step<NBLK>(s.ahead2, A2, c + 1, NB2 * KS2, time2, G, p.by_ctas);
   const int first2 = s_begin / p.by_steps2, n1 = u_end - u_begin, n2 = s_end > s_begin ? (s_end - 1) / p.by_steps2 - first2 + 1 : 0;      // units here
 
   if (warp == MT_BOTH / 32) {
@@ -521,13 +541,13 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     };
     int m = 0;
     // units [from, from + units) of a product, their stages from js0 in the first to js1 in the last
-    auto product = [&](const CUtensorMap* v, const CUtensorMap* sc, const CUtensorMap* vt, const CUtensorMap* st, int NB, const Div& by, int NT, int KT, int KS, int from,
+    auto product = [&](auto expert, const CUtensorMap* v, const CUtensorMap* sc, const CUtensorMap* vt, const CUtensorMap* st, int NB, const Div& by, int NT, int KT, int KS, int from,
                        int units, int js0, int js1) {
       const uint32_t whole = MT_STAGE_KT * MT_UNIT * 68, tail = (uint32_t)((KT - (KS - 1) * MT_STAGE_KT) * MT_UNIT * 68);
       int place = from / by, nb = from - place * NB;
 #pragma unroll 1
       for (int i = 0; i < units && ok; ++i, ++m) {
-        const int tile = (s.act[place] * NT + (nb >> 2)) * KT, end = i + 1 == units ? js1 : KS;
+        const int tile = (expert(place) * NT + (nb >> 2)) * KT, end = i + 1 == units ? js1 : KS;
 #pragma unroll 1
         for (int js = i == 0 ? js0 : 0; js < end && ok; ++js) {
           if (js < KS - 1) stage(m & 1, v, sc, whole, nb, tile + js * MT_STAGE_KT);
@@ -536,8 +556,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         if (++nb == NB) { nb = 0; ++place; }
       }
     };
-    product(&maps.v1, &maps.s1, &maps.v1t, &maps.s1t, NB1, p.by_units1, NT1, KT1, KS1, u_begin, n1, 0, KS1);
-    product(&maps.v2, &maps.s2, &maps.v2t, &maps.s2t, NB2, p.by_units2, NT2, KT2, KS2, first2, n2, s_begin - first2 * KS2, s_end - (first2 + n2 - 1) * KS2);
+    product([&](int at) { return (int)s.act[at]; }, &maps.v1, &maps.s1, &maps.v1t, &maps.s1t, NB1, p.by_units1, NT1, KT1, KS1, u_begin, n1, 0, KS1);
+    product([&](int at) { return s.entries[at] & 255; }, &maps.v2, &maps.s2, &maps.v2t, &maps.s2t, NB2, p.by_units2, NT2, KT2, KS2, first2, n2, s_begin - first2 * KS2, s_end - (first2 + n2 - 1) * KS2);
     if (!ok) __nanosleep(500000);                             // copies in flight land before the block's shared memory goes
     return;
   }
@@ -621,17 +641,17 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
     int have = -1, changes = -1;
 #pragma unroll 1
     for (int m = n1; m < n1 + n2; ++m) {
-      const int u = first2 + m - n1, place = u / p.by_units2, e = s.act[place], n = __popc(s.tokens[e]), lane_row = tid & 31;
-      if (e != have) { have = e; ++changes; }
+      const int u = first2 + m - n1, place = u / p.by_units2, lane_row = tid & 31;
+      const Entry en = entry_of<NBLK>(s, place);
+      const int e = en.e, n = en.n;
+      if (place != have) { have = place; ++changes; }
       mbar_wait_short(SUMS(m & 1), (m >> 1) & 1u, ctl, 1005);
       for (int r = tid >> 5; r < n; r += MT_EPILOGUE / 32) {
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < MT_SHARES; ++w) v += s_red[m & 1][w][r * MT_RED_LD + lane_row];
-        if (two_terms(n, NBLK)) {
 #pragma unroll
-          for (int w = 0; w < MT_SHARES; ++w) v += s_red[m & 1][w][(n + r) * MT_RED_LD + lane_row];
-        }
+        for (int w = 0; w < MT_SHARES; ++w) v += s_red[m & 1][w][(n + r) * MT_RED_LD + lane_row];
         __stcg(p.part + ((int64_t)(u + c) * p.T + r) * MT_UNIT + lane_row, settle(v, p.s2, e, NT2, KT2, (u - place * NB2) * MT_UNIT + lane_row) * s.undo2[changes & 3][r]);
       }
       __syncwarp();
@@ -707,33 +727,33 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
   };
 
   // ---- all units, fc1's and fc2's ----
-  int have = -1, changes = -1;          // expert whose rows of fc2 are staged
-  int n_blocks = 1;                     // of the expert's tokens as columns
-  int place = u_begin / p.by_units1, rest = u_begin - place * NB1;   // the unit's expert in the list of active ones, its place among the expert's units
+  int have = -1, changes = -1;          // entry whose rows of fc2 are staged
+  int n_blocks = 1;                     // of the columns
+  int place = u_begin / p.by_units1, rest = u_begin - place * NB1;   // the unit's active expert or entry, its place among that one's units
 #pragma unroll 1
   for (int m = 0; m < n1 + n2; ++m, ++rest) {
     const bool one = m < n1;
     if (m == n1) { place = first2 / p.by_units2; rest = first2 - place * NB2; }
     if (rest == (one ? NB1 : NB2)) { rest = 0; ++place; }
-    const int e = s.act[place], KT = one ? KT1 : KT2;
+    const int KT = one ? KT1 : KT2;
     const int js0 = m == n1 ? s_begin - first2 * KS2 : 0, js1 = one ? KS1 : m + 1 == n1 + n2 ? s_end - (first2 + n2 - 1) * KS2 : KS2;
-    const uint32_t mask = s.tokens[e];
     if (one) {
-      n_blocks = __popc(mask) > 8 ? 2 : 1;                    // fc1's columns are the expert's tokens among those of the batch
+      const int e = s.act[place];
+      n_blocks = __popc(s.tokens[e]) > 8 ? 2 : 1;             // fc1's columns are the expert's tokens among those of the batch
 #pragma unroll
       for (int b = 0; b < NBLK; ++b) {
         const int t = s.who[e][b * 8 + qrow] & (MT_MAX_TOKENS - 1);      // (any column stands in for one without a token)
         col[b] = (uint32_t)((t >> 3) * 512 + (t & 7) * 64) & (uint32_t)(NBLK * 512 - 1);
       }
-    } else if (e != have) {
-      if (tid == 0) wait_count(p.done1 + e, NB1, ctl, 1003);
+    } else if (place != have) {
+      const Entry en = entry_of<NBLK>(s, place);
+      if (tid == 0) wait_count(p.done1 + en.e, NB1, ctl, 1003);
       bar_sync(1, MT_CONSUMERS);                              // fc1's rows are there, and the staged ones have been read
-      const int n = __popc(mask);
       ++changes;
-      stage_h(p, s, NBLK, toks, e, n, KT2, changes & 3, warp);
+      stage_h(p, s, NBLK, toks, en, KT2, changes & 3, warp);
       bar_sync(1, MT_CONSUMERS);
-      have = e;
-      n_blocks = (two_terms(n, NBLK) ? 2 * n : n) > 8 ? 2 : 1;
+      have = place;
+      n_blocks = 2 * en.n > 8 ? 2 : 1;
 #pragma unroll
       for (int b = 0; b < NBLK; ++b) col[b] = (uint32_t)(b * 512 + qrow * 64);
     }
@@ -781,15 +801,16 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
         c0[x] = c1[x] = 0;
         part[x] = nullptr;
         if (j0 + x < p.k) {
-          const int e = s.sel[t][j0 + x], u = (int)s.rank[e] * NB2 + nb, r = __popc(s.tokens[e] & ((1u << t) - 1u));
+          const int e = s.sel[t][j0 + x], all = __popc(s.tokens[e] & ((1u << t) - 1u)), second = all >= 4 * NBLK ? 1 : 0, r = all - second * 4 * NBLK;
+          const int place = s.from[e] + second, u = place * NB2 + nb;
           // the CTAs whose ranges the unit's first and last stage are in
-          c0[x] = cta_of<NBLK, 16>(s, u * KS2, s.rank[e], NB2 * KS2, time2, G);
-          c1[x] = cta_of<NBLK, 16>(s, u * KS2 + KS2 - 1, s.rank[e], NB2 * KS2, time2, G);
+          c0[x] = cta_of<NBLK>(s.ahead2, u * KS2, place, NB2 * KS2, time2, G);
+          c1[x] = cta_of<NBLK>(s.ahead2, u * KS2 + KS2 - 1, place, NB2 * KS2, time2, G);
           part[x] = p.part + ((int64_t)u * p.T + r) * MT_UNIT + lane;
           if (p.b2) b[x] = load_bias(p.b2, p.b2_dtype, e * p.ld_b2 + o);
         }
       }
-      wait_count(p.done2 + nb, A * KS2, ctl, 1004);
+      wait_count(p.done2 + nb, A2 * KS2, ctl, 1004);
       __syncwarp();
       // the first part and the last, most often all there are, side by side
       float last[4];
@@ -802,9 +823,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tokens_kernel(const TokensP
       for (int x = 0; x < 4; ++x) {
         if (j0 + x >= p.k) break;
         if (c1[x] > c0[x] + 1) {
-          const int place = s.rank[s.sel[t][j0 + x]];
+          const int e = s.sel[t][j0 + x], place = s.from[e] + (__popc(s.tokens[e] & ((1u << t) - 1u)) >= 4 * NBLK ? 1 : 0);
           for (int q = 1, was = c0[x]; q < KS2 - 1; ++q) {
-            const int cc = cta_of<NBLK, 16>(s, (place * NB2 + nb) * KS2 + q, place, NB2 * KS2, time2, G);
+            const int cc = cta_of<NBLK>(s.ahead2, (place * NB2 + nb) * KS2 + q, place, NB2 * KS2, time2, G);
             if (cc != was && cc != c1[x]) v[x] += __ldcg(part[x] + (int64_t)cc * p.T * MT_UNIT);
             was = cc;
           }
@@ -861,12 +882,12 @@ TokensWorkspace mt_workspace(const MoeTokensArgs& a) {
   TokensWorkspace w;
   size_t at = 0;
   auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
-  const int64_t n = (int64_t)a.T * a.k, active = n < a.E ? n : a.E;
+  const int64_t n = (int64_t)a.T * a.k, entries = n < 2 * a.E ? n : 2 * a.E;       // of fc2: two of an expert at most, each of a pick at least
   w.counters = take(3 * MT_COUNTERS * 4);
   w.logits = take((size_t)a.T * a.E * 4);
   w.xmax = take((size_t)a.T * 4);
   w.h = take((size_t)(n * a.ff) * 4);
-  w.part = take((size_t)((active * (a.d / MT_UNIT) + moe_sm_count()) * a.T) * MT_UNIT * 4);
+  w.part = take((size_t)((entries * (a.d / MT_UNIT) + moe_sm_count()) * a.T) * MT_UNIT * 4);
   w.bytes = at;
   return w;
 }
