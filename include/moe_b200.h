@@ -37,7 +37,7 @@ enum { MOE_GEMM_AUTO = 0, MOE_GEMM_SIMT = 1, MOE_GEMM_TCGEN05 = 2, MOE_GEMM_TCGE
        MOE_GEMM_MX_F4 = 7 };     /* ... bf16 tokens as four e2m1 terms (kind::mxf4), blocks of at most 32 rows */
 
 const char* moe_last_error(void);
-int moe_abi_version(void);
+int moe_abi_version(void);        /* 2: MoeLoraArgs ends with `ranks` */
 /* Kernels this library has launched in the calling process so far (every launch site counts itself).  Callers
  * use differences of it, e.g. to count the launches of one step. */
 uint64_t moe_launch_count(void);
@@ -382,7 +382,8 @@ int moe_layer_tokens(const MoeTokensArgs* args, void* stream);
  * y_t = x_t W + bias + scale[a] (x_t A_a) B_a with a = indx[t]; an index that is no adapter (negative, or >= n_adapters) leaves the second part out.
  * x [T, K], y [T, N], w_t (W transposed, [N, K]) and the adapters in one 16-bit type (dtype: bf16 or fp16), sums in fp32, y rounded once.  An adapter's ranks,
  * padded with zeros to a multiple of 16, are pieces of 16: `first` [n_adapters + 1] (device) numbers them through, max_pieces is the largest count
- * of one adapter.  `a`: the pieces' 16 rows of K each, pitch ld_a >= K rounded up to 8, zeros past K.  `b`: per piece [N rounded up to 128 / 8][2][8][8]:
+ * of one adapter; `ranks` [n_adapters] (device): how many ranks each has without the padding, or NULL: whole pieces (an infinite x times a padded row of A is
+ * NaN then).  `a`: the pieces' 16 rows of K each, pitch ld_a >= K rounded up to 8, zeros past K.  `b`: per piece [N rounded up to 128 / 8][2][8][8]:
  * value [g][h][r][c] is B's rank 8 h + c at output 8 g + r, zero past N; finite (the product of a block of tokens multiplies other
  * adapters' B by zero).  x, w_t, a: 16-byte aligned rows, x's padded to 8 values (of any finite contents past K where adapters are given).
  * bias (fp32, fp16 or bf16) and, with n_adapters = 0, everything of the adapters may be NULL.  workspace: 256-byte aligned,
@@ -401,6 +402,7 @@ typedef struct {
   void* y; int64_t ld_y;
   void* workspace; size_t workspace_bytes;
   int32_t* status;
+  const int32_t* ranks;
 } MoeLoraArgs;
 size_t moe_lora_matmul_workspace_bytes(const MoeLoraArgs* args);
 int moe_lora_matmul(const MoeLoraArgs* args, void* stream);

@@ -322,3 +322,27 @@ def test_refusals_of_the_c_entry_point():
     assert lib.moe_lora_matmul_workspace_bytes(None) == 0
     blank = (ctypes.c_uint8 * 512)()
     assert lib.moe_lora_matmul(ctypes.addressof(blank), None) == 1 and b"positive" in lib.moe_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,ranks", [(1, [5]), (1, [16, 7]), (1, [17, 40]), (10, [1, 24, 16]), (300, [1, 24, 16]), (4100, [3, 20])])
+def test_infinities_keep_their_sign_whatever_the_rank(T, ranks, dtype):
+    """Where the signs of x W and of every rank's share agree, a row with an infinite element is infinite with that sign: ranks that an adapter does not have add nothing."""
+    x, w, b, la, lb, scale = make(T, 256, 200, ranks, dtype, 31)
+    sign = torch.where(torch.arange(200, device="cuda") % 3 == 0, -1.0, 1.0).to(dtype)
+    w[9] = (w[9].abs() + 0.01) * sign
+    for a in la:
+        a[9] = a[9].abs() + 0.01
+    lb = [(q.abs() + 0.01) * sign for q in lb]
+    indx = (torch.arange(T, device="cuda") % (len(ranks) + 1)).to(torch.int32) if T > 1 else torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = x.clone()
+    rows = torch.arange(0, T, 3, device="cuda")
+    x[rows, 9] = torch.where(rows % 2 == 0, float("inf"), float("-inf")).to(dtype)
+    pw, adapters = tb.prepare_projection_weight(w), tb.prepare_lora_adapters(la, lb, scale)
+    y = tb.matmul_lora(x, pw, b, adapters, indx)
+    tb.matmul_check_status()
+    assert torch.equal(y[rows], x[rows, 9:10] * sign)
+    others = torch.ones(T, dtype=torch.bool, device="cuda")
+    others[rows] = False
+    assert torch.equal(y[others], tb.matmul_lora(want, pw, b, adapters, indx)[others])

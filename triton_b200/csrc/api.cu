@@ -29,7 +29,7 @@ void moe_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 extern "C" __attribute__((visibility("default"))) uint64_t moe_launch_count(void) { return g_launches.load(); }
 
 extern "C" __attribute__((visibility("default"))) const char* moe_last_error(void) { return g_err; }
-extern "C" __attribute__((visibility("default"))) int moe_abi_version(void) { return 1; }
+extern "C" __attribute__((visibility("default"))) int moe_abi_version(void) { return 2; }
 
 extern "C" __attribute__((visibility("default"))) int moe_device_info(int device, MoeDeviceInfo* out) {
   MOE_CHECK_ARG(out != nullptr, "moe_device_info: out is NULL");

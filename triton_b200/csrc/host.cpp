@@ -377,7 +377,7 @@ Tensor moe_tokens(const Tensor& x_, const Tensor& wg, const OptTensor& bg, int64
 }
 
 // ---- a shared projection with low-rank adapters --------------------------------------------------------------------
-// w in the kernel's memory order; adapters: (a, b, first, scale, adapters, most pieces of one) or None, then indx too
+// w in the kernel's memory order; adapters: (a, b, first, scale, adapters, most pieces of one, ranks or None) or None, then indx too
 Tensor lora(const Tensor& x_, const Tensor& w, const OptTensor& bias, const py::object& adapters, const OptTensor& indx_, const Tensor& status) {
   need_cuda(x_);
   const c10::cuda::CUDAGuard guard(x_.device());
@@ -396,7 +396,7 @@ Tensor lora(const Tensor& x_, const Tensor& w, const OptTensor& bias, const py::
   g.x = x.data_ptr(); g.dtype = dtype_code(x); g.ld_x = T > 1 ? x.stride(0) : K8; g.T = T; g.K = (int)K; g.N = (int)N;
   g.w_t = w.data_ptr(); g.ld_w = N > 1 ? w.stride(1) : K8;
   if (bias) { same_device(x, *bias, "bias"); g.bias = bias->data_ptr(); g.bias_dtype = dtype_code(*bias); }
-  Tensor a, b, first, scale, indx;
+  Tensor a, b, first, scale, ranks, indx;
   if (!adapters.is_none()) {
     const py::tuple t = adapters;
     a = t[0].cast<Tensor>(); b = t[1].cast<Tensor>(); first = t[2].cast<Tensor>(); scale = t[3].cast<Tensor>();
@@ -405,6 +405,11 @@ Tensor lora(const Tensor& x_, const Tensor& w, const OptTensor& bias, const py::
     g.a = a.data_ptr(); g.ld_a = a.size(1); g.b = b.data_ptr(); g.first = first.data_ptr<int32_t>(); g.scale = scale.data_ptr<float>();
     g.n_adapters = t[4].cast<int>(); g.max_pieces = t[5].cast<int>();
     g.indx = indx.data_ptr<int32_t>();
+    if (!t[6].is_none()) {
+      ranks = t[6].cast<Tensor>();
+      same_device(x, ranks, "an adapter");
+      g.ranks = ranks.data_ptr<int32_t>();
+    }
   }
   Tensor y = empty({T, N}, x.scalar_type(), x), ws;
   if (y.numel() == 0) return y;

@@ -31,6 +31,7 @@ struct LoraParams {
   const void* a; int64_t ld_a;
   const uint8_t* b;
   const int32_t* first; const float* scale; int n_adapters, max_pieces;
+  const int32_t* ranks;                                // of every adapter, or NULL: whole pieces
   const int32_t* indx;
   float* t; int64_t ld_t; int t_parts; int64_t t_part_stride;     // shares of k whose sums make up t
   void* y; int64_t ld_y;
@@ -160,6 +161,7 @@ __global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_ke
   for (int l = place; l < count; l += places) {
     const int a = NB == 1 ? only : s_list[l], f = p.first[a];
     const float scale = p.scale[a];                           // (asked for here: behind the sums its trip to memory would be one more)
+    const int ranks = p.ranks ? p.ranks[a] : LR_PIECE * p.max_pieces;
     if ((int)blockIdx.y >= p.first[a + 1] - f) continue;      // (uniform)
     const T16* ra = (const T16*)p.a + (int64_t)(f + blockIdx.y) * LR_PIECE * p.ld_a;
     float acc[NB][4];
@@ -203,7 +205,8 @@ __global__ void __launch_bounds__(SH_WARPS * 32, NB == 1 ? 3 : 2) lora_shrink_ke
       float v = 0.0f;
 #pragma unroll
       for (int w = 0; w < SH_WARPS; ++w) v += s_sum[w][n][ln][j];
-      p.t[part * p.t_part_stride + (row0 + token) * p.ld_t + blockIdx.y * LR_PIECE + rank] = v * scale;
+      // A rank that the adapter does not have adds nothing: its row of zeros times an infinity would be NaN, and NaN times B's zeros too
+      p.t[part * p.t_part_stride + (row0 + token) * p.ld_t + blockIdx.y * LR_PIECE + rank] = (int)blockIdx.y * LR_PIECE + rank < ranks ? v * scale : 0.0f;
     }
     __syncthreads();
   }
@@ -515,6 +518,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
         const int k1 = min(kt1 * BLOCK_K, (p.K + 7) & ~7), r = (warp - 2) * 2;
         const T16 *a = (const T16*)p.a + ((int64_t)s_first[0] * LR_PIECE + r) * p.ld_a, *x = (const T16*)p.x;
         const float scale = p.scale[s_idx[0]];
+        const int ranks = p.ranks ? p.ranks[s_idx[0]] : LR_PIECE;
         float v[2] = {0.0f, 0.0f};
 #pragma unroll 2
         for (int k = kt0 * BLOCK_K + lane * 8; k < k1; k += 256) {
@@ -531,7 +535,7 @@ lora_stream_kernel(const LoraParams p, const StreamPlan pl, const __grid_constan
           v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
           v[1] += __shfl_xor_sync(0xFFFFFFFFu, v[1], o);
         }
-        if (lane < 2) s_t[r + lane] = (lane ? v[1] : v[0]) * scale;
+        if (lane < 2) s_t[r + lane] = r + lane < ranks ? (lane ? v[1] : v[0]) * scale : 0.0f;      // (as in the shrink kernel)
       }
       adapter_bar();
     }
@@ -1104,7 +1108,7 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
   p.bias = a.bias; p.bias_dtype = a.bias_dtype;
   if (adapters) {
     p.a = a.a; p.ld_a = a.ld_a; p.b = (const uint8_t*)a.b; p.first = a.first; p.scale = a.scale; p.n_adapters = a.n_adapters; p.max_pieces = a.max_pieces;
-    p.indx = a.indx;
+    p.ranks = a.ranks; p.indx = a.indx;
     p.t = (float*)a.workspace; p.ld_t = (int64_t)a.max_pieces * LR_PIECE; p.t_parts = sp.parts; p.t_part_stride = a.T * p.ld_t;
   }
   p.y = a.y; p.ld_y = a.ld_y; p.status = a.status;

@@ -26,6 +26,7 @@ class LoraAdapters:
     max_pieces: int         # of one adapter
     d_in: int
     d_out: int
+    ranks_device: torch.Tensor | None = None        # `ranks` as int32 [adapters]; None: whole pieces
 
     @property
     def n_adapters(self):
@@ -65,8 +66,9 @@ def prepare_lora_adapters(a: Sequence[torch.Tensor], b: Sequence[torch.Tensor], 
         wrong = [i for i, bi in enumerate(b) if not bool(torch.isfinite(bi).all())]
         raise ValueError(f"prepare_lora_adapters: b of adapters {wrong} has values that are not finite")
     pb = pb.view(first[-1], 2, 8, groups, 8).permute(0, 3, 1, 4, 2).contiguous()
-    return LoraAdapters(pa, pb, torch.tensor(first, dtype=torch.int32, device=device),
-                        torch.tensor([float(s) for s in scale], dtype=torch.float32, device=device), ranks, max(pieces), d_in, d_out)
+    counts = torch.tensor([*first, *ranks], dtype=torch.int32, device=device)
+    return LoraAdapters(pa, pb, counts[:len(first)], torch.tensor([float(s) for s in scale], dtype=torch.float32, device=device), ranks, max(pieces), d_in, d_out,
+                        counts[len(first):])
 
 
 def prepare_projection_weight(w: torch.Tensor) -> torch.Tensor:
@@ -109,5 +111,6 @@ def matmul_lora(x: torch.Tensor, w: torch.Tensor, bias, adapters: LoraAdapters |
             raise ValueError(f"matmul_lora: adapters are [{adapters.d_in}, r] x [r, {adapters.d_out}] of {adapters.a.dtype}, the projection [{K}, {N}] of {x.dtype}")
         if indx.ndim != 1 or indx.shape[0] != T or indx.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"matmul_lora: indx is a vector of {T} int32 or int64")
-        packed = (adapters.a, adapters.b, adapters.first, adapters.scale, adapters.n_adapters, adapters.max_pieces)
+        packed = (adapters.a, adapters.b, adapters.first, adapters.scale, adapters.n_adapters, adapters.max_pieces,
+                  adapters.ranks_device)
     return _lib.host().lora(x, prepare_projection_weight(w), bias, packed, indx, _status_word(x.device))
