@@ -380,7 +380,8 @@ int moe_layer_tokens(const MoeTokensArgs* args, void* stream);
 
 /* ---- a shared projection with low-rank adapters of many requests ---------------------------------
  * y_t = x_t W + bias + scale[a] (x_t A_a) B_a with a = indx[t]; an index that is no adapter (negative, or >= n_adapters) leaves the second part out.
- * x [T, K], y [T, N], w_t (W transposed, [N, K]) and the adapters in one 16-bit type (dtype: bf16 or fp16), sums in fp32, y rounded once.  An adapter's ranks,
+ * x [T, K], y [T, N], w_t (W transposed, [N, K]) and the adapters in one 16-bit type (dtype: bf16 or fp16), sums in fp32, y rounded once; x_t A_a enters the second
+ * product in fp32, with more than 128 tokens in bf16 as two bf16 terms (2^-17 of a value off).  An adapter's ranks,
  * padded with zeros to a multiple of 16, are pieces of 16: `first` [n_adapters + 1] (device) numbers them through, max_pieces is the largest count
  * of one adapter; `ranks` [n_adapters] (device): how many ranks each has without the padding, or NULL: whole pieces (an infinite x times a padded row of A is
  * NaN then).  `a`: the pieces' 16 rows of K each, pitch ld_a >= K rounded up to 8, zeros past K.  `b`: per piece [N rounded up to 128 / 8][2][8][8]:

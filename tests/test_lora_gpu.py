@@ -346,3 +346,30 @@ def test_infinities_keep_their_sign_whatever_the_rank(T, ranks, dtype):
     others = torch.ones(T, dtype=torch.bool, device="cuda")
     others[rows] = False
     assert torch.equal(y[others], tb.matmul_lora(want, pw, b, adapters, indx)[others])
+
+
+@gpu
+@pytest.mark.parametrize("scale,size", [(4.0e4, 2.0 ** -10), (1.0e-6, 2.0 ** 9), (1.0, 1.0)])
+@pytest.mark.parametrize("T,N,ranks", [(128, 136, [16, 40, 5]), (129, 136, [16, 40, 5]), (300, 500, [16, 40, 5]), (1500, 900, [16, 40, 5]), (600, 200, [1000, 64])])
+def test_x_a_outside_the_range_of_fp16(T, N, ranks, scale, size):
+    """scale * x A of 1e5 and of 1e-6, beside B's that bring y back into range, in fp16: as with values near one, on both sides of 128 tokens.  x A is 24 bits there, of products
+    that stay exact; what is left out of them is below 2^-22."""
+    x, _, b, la, lb, _ = make(T, 96, N, ranks, torch.float16, 41)
+    w = torch.zeros(96, N, device="cuda", dtype=torch.float16)
+    lb = [(q.double() * size).half() for q in lb]
+    scales = [scale * (1 + i) for i in range(len(ranks))]
+    indx = indices(T, len(ranks), "random", 41)
+    y = tb.matmul_lora(x, tb.prepare_projection_weight(w), None, tb.prepare_lora_adapters(la, lb, scales), indx)
+    tb.matmul_check_status()
+    ref, bound = torch.zeros(T, N, dtype=torch.float64, device="cuda"), torch.zeros(T, N, dtype=torch.float64, device="cuda")
+    most = 0.0
+    for i, (a, q, s) in enumerate(zip(la, lb, scales)):
+        at = torch.nonzero(indx == i).squeeze(1)
+        t = s * (x[at].double() @ a.double())
+        e_t = s * (96 / 16 + 32) * 2.0 ** -23 * (x[at].abs().double() @ a.abs().double()) + 2.0 ** -22 * t.abs()
+        ref[at] = t @ q.double()
+        bound[at] = e_t @ q.double().abs() + ((96 + 5 * a.shape[1]) / 16 + 32) * 2.0 ** -23 * (t.abs() @ q.double().abs())
+        most = max(most, t.abs().max().item())
+    assert ref.abs().max() < 6e4 and (most > 65504 or scale < 4e4)
+    bound += (ref.abs() + bound) * 2.0 ** -11 + 2.0 ** -25              # (half a step of fp16, or of its subnormals)
+    check(y, ref, bound)

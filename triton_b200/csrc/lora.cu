@@ -7,8 +7,8 @@
 //     has, on mma.sync with operands straight from global memory: there are 16 ranks, too few for a tcgen05 operand of 128 rows, and at single
 //     tokens reading A is all there is to do.
 //  2. the product: W's tiles and x's through a ring by TMA, tcgen05.mma.kind::f16 into fp32 in tensor memory; then, into the same accumulator, one MMA per
-//     piece and term: B's tile times the tokens' t, zero for the tokens of other adapters, so that a block of tokens may hold any mixture.  t enters in two
-//     terms (hi + lo, 16 bits of it in bf16), so it costs the result nothing.
+//     piece and term: B's tile times the tokens' t, zero for the tokens of other adapters, so that a block of tokens may hold any mixture.  t enters in bf16
+//     terms, two (17 bits of it) for bf16, three for fp16, whose B is two bf16 parts then: see "pieces as MMA operands".
 // The second has two forms: lora_stream_kernel for few tokens, whose adapters' part runs on CUDA cores beside the product (one token's first part too), and
 // lora_pair_kernel for many, as above.
 // Measured, K = 2880, N = 5120, shrink + product: 1 token 9.3 us of one launch (29.7 MB at 3.2 TB/s; its start, the first loads and the meeting of the shares of
@@ -221,16 +221,45 @@ constexpr uint32_t PIECE_DESC_HI = (256u >> 4) | (1u << 14);            // strid
 __device__ __forceinline__ uint32_t lr_idesc(bool f16, int m, int n) {
   return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-template <typename T16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  T16 h[2] = {from_f32<T16>(a), from_f32<T16>(b)};
+// A piece as operands.  bf16: B's tile, and t in two terms (17 bits of it, 2^-17 of a value: the result keeps 8).  fp16: its range ends at 65504 and its steps
+// at 2^-24, t's do not, and an MMA's operands have one type.  So both go in as bf16, which has fp32's range: t in three terms, all of its 24 bits; a value of
+// B, which has 11, in two tiles.  B's second tile times t's third term is left out, 2^-23 of a product.
+template <typename T16> constexpr bool LR_F16 = std::is_same<T16, __half>::value;
+constexpr int lr_tiles(bool f16) { return f16 ? 2 : 1; }
+constexpr int lr_terms(bool f16) { return f16 ? 3 : 2; }
+constexpr int lr_piece_bytes(bool f16, int tb) { return lr_tiles(f16) * LR_PIECE_BYTES + lr_terms(f16) * tb * 16; }     // of one CTA: half of the block's tokens
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  __nv_bfloat16 h[2] = {__float2bfloat16_rn(a), __float2bfloat16_rn(b)};
   return *reinterpret_cast<const uint32_t*>(h);
 }
-// Sixteen ranks of token row `row` (of the block; `live`: it has this adapter) as row `at` of the operand: high terms at dst, what they leave at dst + lo
+// what bf16 has of a value, rounded (two terms) or cut off (three: the rest of a sum of cut-off terms is exact); all of one that is not finite
+template <bool CUT> __device__ __forceinline__ float bf16_term(float v) {
+  return CUT && isfinite(v) ? __uint_as_float(__float_as_uint(v) & 0xFFFF0000u) : __bfloat162float(__float2bfloat16_rn(v));
+}
+// Eight fp16 values -> their two bf16 parts.  Both have the value's sign and, but for a zero, neither is zero, so that an infinite t times the two is infinite with that
+// sign: where the leading eight bits are all there is, a step of them goes to the second part.
+__device__ __forceinline__ void split_f16(const uint4& v, uint4& hi, uint4& lo) {
+  const __half* e = reinterpret_cast<const __half*>(&v);
+  uint32_t h[8], l[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float f = __half2float(e[j]);
+    const uint32_t u = __float_as_uint(f);
+    h[j] = (u & 0x7FFFFFFFu) == 0u ? u : (u & 0xFFFF0000u) - ((u & 0xFFFFu) == 0u ? 0x10000u : 0u);
+    l[j] = __float_as_uint(f - __uint_as_float(h[j]));
+  }
+  hi = make_uint4(h[0] >> 16 | h[1], h[2] >> 16 | h[3], h[4] >> 16 | h[5], h[6] >> 16 | h[7]);
+  lo = make_uint4(l[0] >> 16 | l[1], l[2] >> 16 | l[3], l[4] >> 16 | l[5], l[6] >> 16 | l[7]);
+}
+// Sixteen ranks of a token (`live`: it has this adapter) as row `at` of the operand: the first terms at dst, what each leaves `step` bytes on
 template <typename T16>
-__device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, int64_t token, int rank0, uint32_t dst, uint32_t lo, int at) {
-  uint4 h[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, l[2] = {h[0], h[0]};
+__device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, int64_t token, int rank0, uint32_t dst, uint32_t step, int at) {
+  constexpr int TERMS = lr_terms(LR_F16<T16>);
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.0f;
   if (live) {
-    float v[16];
     const float4* src = reinterpret_cast<const float4*>(p.t + token * p.ld_t + rank0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -243,23 +272,22 @@ __device__ __forceinline__ void write_piece_row(const LoraParams& p, bool live, 
         const float4 q = *(reinterpret_cast<const float4*>(p.t + s * p.t_part_stride + token * p.ld_t + rank0) + i);
         v[4 * i] += q.x; v[4 * i + 1] += q.y; v[4 * i + 2] += q.z; v[4 * i + 3] += q.w;
       }
-    float left[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float d = v[i] - to_f32<T16>(from_f32<T16>(v[i]));
-      left[i] = isfinite(d) ? d : 0.0f;                       // infinities and NaN are the first term's
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      h[i] = make_uint4(pack2<T16>(v[8 * i], v[8 * i + 1]), pack2<T16>(v[8 * i + 2], v[8 * i + 3]), pack2<T16>(v[8 * i + 4], v[8 * i + 5]), pack2<T16>(v[8 * i + 6], v[8 * i + 7]));
-      l[i] = make_uint4(pack2<T16>(left[8 * i], left[8 * i + 1]), pack2<T16>(left[8 * i + 2], left[8 * i + 3]), pack2<T16>(left[8 * i + 4], left[8 * i + 5]), pack2<T16>(left[8 * i + 6], left[8 * i + 7]));
-    }
   }
   const uint32_t to = dst + (uint32_t)((at >> 3) * 256 + (at & 7) * 16);
-  sts128(to, h[0]);
-  sts128(to + 128, h[1]);
-  sts128(to + lo, l[0]);
-  sts128(to + lo + 128, l[1]);
+#pragma unroll
+  for (int term = 0; term < TERMS; ++term) {
+    float h[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      h[i] = bf16_term<TERMS == 3>(v[i]);
+      const float d = v[i] - h[i];
+      v[i] = isfinite(d) ? d : 0.0f;                          // infinities and NaN are the first term's
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      sts128(to + (uint32_t)term * step + (uint32_t)i * 128u,
+             make_uint4(pack_bf16(h[8 * i], h[8 * i + 1]), pack_bf16(h[8 * i + 2], h[8 * i + 3]), pack_bf16(h[8 * i + 4], h[8 * i + 5]), pack_bf16(h[8 * i + 6], h[8 * i + 7])));
+  }
 }
 
 // whether the word at this place is zero in the first n CTAs of the cluster (a lane asks one of them: one after the other they took 2 us)
@@ -652,8 +680,10 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t crank = cluster_ctarank(), half_id = crank & 1u, even = crank & ~1u, both = 3u << even;
   const int S = pl.splits, split = (int)(crank >> 1), TB = pl.tb, n_mma = TB / pl.mmas, half = n_mma / 2;
+  constexpr bool F16 = LR_F16<T16>;
+  constexpr uint32_t B_BYTES = lr_tiles(F16) * LR_PIECE_BYTES;
   const uint32_t X_BYTES = (uint32_t)(TB / 2) * 128u, stage_bytes = SUBTILE_BYTES + X_BYTES, T_BYTES = (uint32_t)(TB / 2) * 32u,
-                 piece_bytes = LR_PIECE_BYTES + 2 * T_BYTES;
+                 piece_bytes = (uint32_t)lr_piece_bytes(F16, TB);
   const uint32_t piece0 = sbase + (uint32_t)pl.stages * stage_bytes;
   auto FULL = [&](int s) { return smem_u32(&bars[s]); };                                   // of the even CTA: both CTAs' tiles
   auto EMPTY = [&](int s) { return smem_u32(&bars[LP_MAX_STAGES + s]); };
@@ -718,7 +748,7 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
       // ================================= MMA ===================================================================
       int it = 0, m = 0;
       bool ok = true;
-      const uint32_t idesc = lr_idesc(std::is_same<T16, __half>::value, 256, n_mma);
+      const uint32_t idesc = lr_idesc(F16, 256, n_mma), idesc_piece = lr_idesc(false, 256, n_mma);
       for (int tile = tile0, tc = 0; tile < tile1 && ok; ++tile, ++tc) {
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(ACC_FREE, (tc & 1u) ^ 1u, ctl, 1113));
         if (!ok) break;
@@ -743,11 +773,14 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
           ok = __all_sync(0xFFFFFFFFu, mbar_wait(PFULL(s), (m / pl.pieces) & 1u, ctl, 1115));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t st = piece0 + (uint32_t)s * piece_bytes, a_lo = piece_desc(st), b_lo = piece_desc(st + LR_PIECE_BYTES);
-          for (int j = 0; j < pl.mmas; ++j) {
-            elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo, b_lo + (uint32_t)(j * half * 2), PIECE_DESC_HI, idesc, 1u);
-            elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo, b_lo + (T_BYTES >> 4) + (uint32_t)(j * half * 2), PIECE_DESC_HI, idesc, 1u);
-          }
+          const uint32_t st = piece0 + (uint32_t)s * piece_bytes, a_lo = piece_desc(st), b_lo = piece_desc(st + B_BYTES);
+          for (int j = 0; j < pl.mmas; ++j)
+#pragma unroll
+            for (int tile_of_b = 0; tile_of_b < lr_tiles(F16); ++tile_of_b)
+#pragma unroll
+              for (int term = 0; term < lr_terms(F16) - tile_of_b; ++term)
+                elect_mma_pair_f16(tmem + (uint32_t)(j * n_mma), a_lo + (uint32_t)tile_of_b * (LR_PIECE_BYTES >> 4),
+                                   b_lo + (uint32_t)term * (T_BYTES >> 4) + (uint32_t)(j * half * 2), PIECE_DESC_HI, idesc_piece, 1u);
           elect_commit_both(PEMPTY(s), both);
         }
         if (ok) elect_commit_both(ACC, both);
@@ -815,12 +848,19 @@ lora_pair_kernel(const LoraParams p, const PairPlan pl, const __grid_constant__ 
           for (int r = (warp - 6) * 32 + lane; r < TB / 2; r += 128) {
             const int j = r >= half ? 1 : 0;
             const int64_t token = (int64_t)block * TB + j * n_mma + (int)half_id * half + (r - j * half);
-            write_piece_row<T16>(p, token < p.T && p.indx[token] == a, token, i * LR_PIECE, dst + LR_PIECE_BYTES, T_BYTES, r);
+            write_piece_row<T16>(p, token < p.T && p.indx[token] == a, token, i * LR_PIECE, dst + B_BYTES, T_BYTES, r);
           }
+          if (F16 || warp == 6) ok = __all_sync(0xFFFFFFFFu, mbar_wait(PTILE(s), (m / pl.pieces) & 1u, ctl, 1117));
+          if (!ok) break;
+          if (F16)                                            // B's tile becomes its two bf16 parts, the first in its place
+            for (uint32_t at = dst + (uint32_t)((warp - 6) * 32 + lane) * 16u; at < dst + LR_PIECE_BYTES; at += 128 * 16u) {
+              uint4 hi, lo;
+              split_f16(lds128(at), hi, lo);
+              sts128(at, hi);
+              sts128(at + LR_PIECE_BYTES, lo);
+            }
           fence_proxy_async();
           __syncwarp();
-          if (warp == 6) ok = __all_sync(0xFFFFFFFFu, mbar_wait(PTILE(s), (m / pl.pieces) & 1u, ctl, 1117));
-          if (!ok) break;
           if (lane == 0) mbar_arrive_cluster(PFULL(s), even);
           ++m;
         }
@@ -953,7 +993,7 @@ int64_t lr_pair_clusters(int s) {
 
 // Form of the product for many tokens.  Tokens are cut into blocks and k over up to four pairs; a round of tiles costs what comes into an SM, in rows of
 // 128 bytes, and draining the accumulator about as much as 2.6 rows a token.
-PairPlan lr_pair_plan(int64_t T, int K, int N) {
+PairPlan lr_pair_plan(int64_t T, int K, int N, bool f16) {
   PairPlan best = {};
   const int64_t KT = cdiv64(K, BLOCK_K), tiles_n = cdiv64(N, 256);
   int64_t side[LP_MAX_SPLITS + 1];                            // clusters of so many pairs that run side by side
@@ -976,10 +1016,12 @@ PairPlan lr_pair_plan(int64_t T, int K, int N) {
     }
   }
   best.mmas = best.tb > 256 ? 2 : 1;
-  const int stage = SUBTILE_BYTES + best.tb * 64, piece = LR_PIECE_BYTES + best.tb * 32, room = 224 * 1024;
-  best.pieces = LP_MAX_PIECES;
-  best.stages = (room - best.pieces * piece) / stage;
+  // Two pieces of fp16, larger ones, at the least, so that they take no stage away that bf16 has
+  const int stage = SUBTILE_BYTES + best.tb * 64, piece = lr_piece_bytes(f16, best.tb), room = 224 * 1024;
+  best.stages = (room - (f16 ? 2 : LP_MAX_PIECES) * piece) / stage;
   if (best.stages > LP_MAX_STAGES) best.stages = LP_MAX_STAGES;
+  best.pieces = (room - best.stages * stage) / piece;
+  if (best.pieces > LP_MAX_PIECES) best.pieces = LP_MAX_PIECES;
   int bytes = best.stages * stage + best.pieces * piece;
   if (best.splits > 1 && bytes < best.tb * LR_TILE_N * 4) bytes = best.tb * LR_TILE_N * 4;
   best.smem = bytes + 1024;
@@ -992,7 +1034,7 @@ PairPlan lr_pair_plan(int64_t T, int K, int N) {
 bool lr_many(int64_t T) { return T > 128; }
 
 size_t lr_t_bytes(const MoeLoraArgs& a, ShrinkPlan s) { return ((size_t)s.parts * (size_t)a.T * (size_t)a.max_pieces * LR_PIECE * 4 + 255) / 256 * 256; }
-size_t lr_list_bytes(const MoeLoraArgs& a) { return lr_many(a.T) ? (size_t)lr_pair_plan(a.T, a.K, a.N).blocks * LR_LIST * 4 : 0; }
+size_t lr_list_bytes(const MoeLoraArgs& a) { return lr_many(a.T) ? (size_t)lr_pair_plan(a.T, a.K, a.N, a.dtype == MOE_F16).blocks * LR_LIST * 4 : 0; }
 
 int lr_check(const MoeLoraArgs* a) {
   MOE_CHECK_ARG(a, "moe_lora_matmul: NULL argument");
@@ -1113,7 +1155,7 @@ extern "C" __attribute__((visibility("default"))) int moe_lora_matmul(const MoeL
   }
   p.y = a.y; p.ld_y = a.ld_y; p.status = a.status;
   const bool many = lr_many(a.T);
-  const PairPlan pl = many ? lr_pair_plan(a.T, a.K, a.N) : PairPlan{};
+  const PairPlan pl = many ? lr_pair_plan(a.T, a.K, a.N, a.dtype == MOE_F16) : PairPlan{};
   if (adapters && many) {
     p.list = (int32_t*)((uint8_t*)a.workspace + lr_t_bytes(a, sp));
     p.list_tb = pl.tb;

@@ -90,8 +90,8 @@ def matmul_lora(x: torch.Tensor, w: torch.Tensor, bias, adapters: LoraAdapters |
     x [T, d_in], w [d_in, d_out] (in the memory order of `prepare_projection_weight`, else it is re-laid-out on every call) and the adapters in one type,
     bf16 or fp16; bias [d_out] or None; indx [T] int32 or int64, any order: a negative index, or one past the last adapter, is a row without an adapter.
     Rows of a request that stand together share the reads of its adapter.  Sums are fp32 and y is rounded once; x a[a] goes into the
-    second product in fp32 or, with more than 128 tokens, in two 16-bit terms (in fp16 it overflows from 65520 on then, as a rounded one would).  `adapters` None (then indx too) is the projection by itself.  Runs on the current stream of x's device, which has
-    to hold all tensors; every call has a workspace of its own, so calls may overlap and be captured in CUDA graphs."""
+    second product in fp32, which with more than 128 tokens in bf16 is two bf16 terms, 2^-17 of a value off.  `adapters` None (then indx too) is the projection by
+    itself.  Runs on the current stream of x's device, which has to hold all tensors; every call has a workspace of its own, so calls may overlap and be captured in CUDA graphs."""
     if not isinstance(x, torch.Tensor) or x.ndim != 2 or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("matmul_lora: x is a [tokens, d_in] tensor of bf16 or fp16")
     if not x.is_cuda:
