@@ -394,3 +394,13 @@ def test_hidden_rows_keep_their_bits_however_many_tokens_an_expert_has(T, E, k, 
 ])
 def test_experts_of_most_tokens(T, E, k, d, ff, dtype):
     run_case(T, E, k, d, ff, dtype, seed=17)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_a_router_weight_that_is_not_bf16_is_refused(dtype):
+    """casting it would round the logits' factors, by which experts are picked, without the caller's knowing"""
+    x, wg, bg, lw, k, _, _ = small()
+    with pytest.raises(ValueError, match="bf16"):
+        tb.moe_layer_tokens(x, wg.to(dtype), bg, lw, k)
+    assert torch.isfinite(tb.moe_layer_tokens(x, tb.prepare_router_weight(wg.to(dtype)), bg, lw, k)).all()

@@ -32,6 +32,8 @@ def moe_layer_tokens(x: torch.Tensor, wg: torch.Tensor, bg, lw: MoeLayerWeights,
     E = lw.n_expts
     if wg.ndim != 2 or tuple(wg.shape) != (d, E):
         raise ValueError(f"moe_layer_tokens: wg is [{d}, {E}] for these tokens and experts, got {list(wg.shape)}")
+    if wg.dtype != torch.bfloat16:
+        raise ValueError(f"moe_layer_tokens: wg is bf16, got {wg.dtype} (prepare_router_weight casts it)")
     if bg is not None and (bg.ndim != 1 or bg.shape[0] != E or bg.stride(0) != 1 or bg.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
         raise ValueError(f"moe_layer_tokens: bg is a contiguous vector of {E} floats")
     if not 0 < k <= E:
