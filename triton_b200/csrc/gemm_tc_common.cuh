@@ -78,6 +78,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const C
   }
 }
 
+// mbar_wait for loops of few instructions: after the tries that a wait most often takes (some 4 us each where nothing comes) the rest is a call.  When the time
+// limit is past, or another wait of the CTA has run out, it returns like one that is over.
+__device__ __noinline__ void mbar_wait_rest(uint32_t bar, uint32_t parity, const Ctl ctl, int code) { mbar_wait(bar, parity, ctl, code); }
+__device__ __forceinline__ void mbar_wait_short(uint32_t bar, uint32_t parity, const Ctl& ctl, int code) {
+  uint32_t tries = 0;
+  while (!mbar_try(bar, parity))
+    if (++tries == 16u) {
+      mbar_wait_rest(bar, parity, ctl, code);
+      break;
+    }
+}
+
 // prefix[1 .. n]: counts of n experts -> counts of the experts up to each, prefix[0] = 0 (one warp).  (By a single thread 128 experts took some 2 us
 // of every launch.)
 __device__ __forceinline__ void warp_prefix(int32_t* prefix, int n, int lane) {

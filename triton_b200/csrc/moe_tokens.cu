@@ -245,19 +245,6 @@ __device__ __forceinline__ bool wait_count(const int32_t* counter, int full, con
     }
   }
 }
-// mbar_wait for the loops of few instructions: what is hardly ever run is a call, and time is counted in tries (each of which may take a while)
-__device__ __noinline__ bool mbar_expired(uint32_t tries, const Ctl ctl, int code) {
-  if (*ctl.abort_flag) return true;
-  if (tries < (1u << 24)) return false;
-  *ctl.abort_flag = 1;
-  if (ctl.status) atomicExch(ctl.status, code);
-  return true;
-}
-__device__ __forceinline__ void mbar_wait_short(uint32_t bar, uint32_t parity, const Ctl& ctl, int code) {
-  uint32_t tries = 0;
-  while (!mbar_try(bar, parity))
-    if ((++tries & 1023u) == 0 && mbar_expired(tries, ctl, code)) break;
-}
 // named barriers: 1 consumers, 2 epilogue, 3 all but those that stage tokens
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int MT_BOTH = MT_CONSUMERS + MT_EPILOGUE;
