@@ -373,3 +373,26 @@ def test_x_a_outside_the_range_of_fp16(T, N, ranks, scale, size):
     assert ref.abs().max() < 6e4 and (most > 65504 or scale < 4e4)
     bound += (ref.abs() + bound) * 2.0 ** -11 + 2.0 ** -25              # (half a step of fp16, or of its subnormals)
     check(y, ref, bound)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("order", ["turns", "random", "runs", "back"])
+@pytest.mark.parametrize("T,K,N,ranks", [
+    # x A goes by blocks of 64 tokens beyond 1024 tokens of more than 3500 tokens times pieces, by eights below: both sides of either line
+    (4500, 300, 136, [1 + i % 16 for i in range(64)]),          # as many adapters in a block as it has tokens
+    (4100, 2001, 200, [16, 3, 40, 24, 8, 17, 64]),              # rows of x that are not 16-byte aligned
+    (1030, 2888, 264, [64, 5, 33, 16, 48, 1]),                  # few blocks: k in four parts
+    (1750, 520, 72, [32, 9, 17]), (1751, 520, 72, [32, 9, 17]),
+    (1024, 1032, 72, [64, 30, 1, 16, 16]), (1025, 1032, 72, [64, 30, 1, 16, 16]),
+    (3501, 96, 40, [7] * 130), (3500, 96, 40, [7] * 130),
+])
+def test_long_batches_of_mixed_adapters(T, K, N, ranks, order, dtype):
+    L = len(ranks)
+    x, w, b, la, lb, scale = make(T, K, N, ranks, dtype, 51)
+    at = torch.arange(T, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(52)
+    indx = {"turns": at % (L + 1) - 1, "random": torch.randint(-1, L + 1, (T,), device="cuda", generator=g), "runs": at * L // T, "back": (L - 1) - at * 37 % L}[order].to(torch.int32)
+    y = tb.matmul_lora(x, tb.prepare_projection_weight(w), b, tb.prepare_lora_adapters(la, lb, scale), indx)
+    tb.matmul_check_status()
+    check(y, *reference(x, w, b, la, lb, scale, indx))
