@@ -396,3 +396,21 @@ def test_long_batches_of_mixed_adapters(T, K, N, ranks, order, dtype):
     y = tb.matmul_lora(x, tb.prepare_projection_weight(w), b, tb.prepare_lora_adapters(la, lb, scale), indx)
     tb.matmul_check_status()
     check(y, *reference(x, w, b, la, lb, scale, indx))
+
+
+def test_prepared_adapters_carry_their_ranks():
+    *_, la, lb, scale = make(1, 20, 130, [3, 17, 16], torch.float16, 0, device="cpu")
+    p = tb.prepare_lora_adapters(la, lb, scale)
+    assert p.ranks_device.tolist() == [3, 17, 16] and p.first.tolist() == [0, 1, 3, 4] and p.ranks_device.dtype == p.first.dtype == torch.int32
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 50, 400])
+def test_adapters_without_ranks_are_whole_pieces(T):
+    import dataclasses
+    x, w, b, la, lb, scale = make(T, 128, 200, [5, 16, 9], torch.bfloat16, 61)
+    pw, adapters, indx = tb.prepare_projection_weight(w), tb.prepare_lora_adapters(la, lb, scale), indices(T, 3, "random", 61)
+    want = tb.matmul_lora(x, pw, b, adapters, indx)
+    assert torch.equal(tb.matmul_lora(x, pw, b, dataclasses.replace(adapters, ranks_device=None), indx), want)
+    with pytest.raises(ValueError):
+        tb.matmul_lora(x, pw, b, dataclasses.replace(adapters, ranks_device=adapters.ranks_device.cpu()), indx)
