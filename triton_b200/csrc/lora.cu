@@ -12,8 +12,8 @@
 // The second has two forms: lora_stream_kernel for few tokens, whose adapters' part runs on CUDA cores beside the product (one token's first part too), and
 // lora_pair_kernel for many, as above.
 // Measured, K = 2880, N = 5120, shrink + product: 1 token 9.3 us of one launch (29.7 MB at 3.2 TB/s; its start, the first loads and the meeting of the shares of
-// k are half), 64 tokens with an adapter each of 1 to 64 ranks 7 + 20 (55 MB), 300 tokens 6.4 + 23, 8192 tokens 18 + 213 (1134 TFLOP/s).  What bounds
-// the last: a CTA takes in 48 KB for 1024 cycles of MMA, and an SM some 32 B a cycle.
+// k are half), 64 tokens with an adapter each of 1 to 64 ranks 7 + 20 (55 MB), 300 tokens 6.4 + 23, 8192 tokens 18 + 213: 231 one call at a time
+// (1.05 PFLOP/s; the product's kernel by itself 1.13), 258 in a long run, whose clock the power limit takes to 1.6 GHz (0.94).  What bounds the last: a CTA takes in 48 KB for 1024 cycles of MMA, and an SM some 32 B a cycle.
 #include "gemm_pair_common.cuh"
 #include <cuda_fp16.h>
 #include <atomic>

@@ -12,13 +12,13 @@
 //     when they are there, and the ring goes on filling with fc2's weights meanwhile (one token of four experts: all of them).
 //     fc2's partial sums go to the workspace; a counter per 32 output columns says when they are complete, and a warp of whichever CTA adds up 32
 //     outputs of a token in a fixed order (slots, then parts along k): the result does not depend on who comes last.
-// Measured, 2880 x 2880, k = 4, 128 experts, router + layer: 1 token 3.7 + 23 us (54 MB), 4 tokens 4.2 + 46 (173 MB, 3.7 TB/s), 16 tokens 4.4 + 106 (398 MB,
-// 3.8 TB/s).  One token: selection 2.2, fc1's first sums 4 later, all of fc1 at 14, its rows staged 1.6 later, fc2 3, the meeting of the sums 2.5.  With more, a
-// stage of 17.4 KB takes an SM 0.5 us (its bytes some 0.4 at the copy bandwidth): instructions, 61 % of issue slots and 53 % of the integer pipe, which the
+// Measured, 2880 x 2880, k = 4, 128 experts, router + layer: 1 token 3.7 + 23 us (54 MB), 4 tokens of 13 experts 4.2 + 48 (173 MB, 3.6 TB/s), 16 tokens of 26 experts
+// 4.4 + 103 (345 MB, 3.3 TB/s), of 35 experts 125 (464 MB, 3.7 TB/s).  One token: selection 2.2, fc1's first sums 4 later, all of fc1 at 14, its rows staged 1.6 later, fc2 3, the meeting of the sums 2.5.  With more, a
+// stage of 17.4 KB takes an SM 0.5 us (its bytes some 0.4 at the copy bandwidth): instructions, 60 % of issue slots and 50 % of the integer pipe, which the
 // conversions of codes and scales are two thirds of; the loads of a warp's second tile ahead of the first one's arithmetic made it 7 % slower.
 //
 // Arithmetic: a code becomes fp16 exactly, tokens are fp16 scaled by their row's largest finite element, which is put in [2^13, 2^14):
-// elements down to 2^-30 of it keep all of bf16's bits.  mma.sync m16n8k16 sums one scale group of 32 k in fp32, which
+// elements down to 2^-30 of it keep all of bf16's bits (27 fp16's), and a sum of more than 2^114 times it is infinite.  mma.sync m16n8k16 sums one scale group of 32 k in fp32, which
 // is multiplied by the group's scale and added up in fp32.  The legacy tensor path is far more than 16 tokens need, and its fragments come straight
 // from the packed words.  SwiGLU outputs stay fp32 in the workspace; as operand they are two fp16 terms of the row's scale, 2^-23 of a value off (2^-38 of
 // the row's largest where it is that small).
@@ -882,6 +882,9 @@ TokensWorkspace mt_workspace(const MoeTokensArgs& a) {
 // the shared memory that is left for the ring, whole stages
 constexpr int MT_SMEM = 232448;
 template <int NBLK> constexpr int mt_static_smem() { return (int)(sizeof(TokensShared) + 2 * MT_SHARES * 8 * NBLK * MT_RED_LD * 4) + 64; }
+
+// four stages at the widest that two blocks of columns take: with two, one a team, a layer of 4096 x 2880 and 16 tokens took 158 us in place of 105
+static_assert(MT_SMEM - mt_static_smem<2>() - 128 - 4096 / 128 * 4 * 512 * 2 >= 4 * MT_STAGE_BYTES, "TokensShared has outgrown its room");
 
 int mt_check(const MoeTokensArgs* a) {
   MOE_CHECK_ARG(a, "moe_layer_tokens: NULL argument");

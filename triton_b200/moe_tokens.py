@@ -21,7 +21,7 @@ def moe_layer_tokens(x: torch.Tensor, wg: torch.Tensor, bg, lw: MoeLayerWeights,
     layouts.  Router logits, all sums and what is between the two products are fp32 (a hidden row enters the second as two fp16 terms, 2^-23 of a value, however many
     tokens its expert has) and the result is rounded once: `moe_layer_forward` on `router_topk`'s selection rounds the logits (by default), the hidden rows and every
     expert's output to bf16 too.  Equal logits go to the lower
-    expert.  At most 256 experts, k <= 16, widths that are multiples of 32 up to 8192 (4096 for more than 8 tokens); NotImplementedError
+    expert.  A sum of more than 2^114 times the largest element of its row is infinite.  At most 256 experts, k <= 16, widths that are multiples of 32 up to 8192 (4096 for more than 8 tokens); NotImplementedError
     beyond.  Runs on the current stream of x's device, which has to hold all tensors; every call has a workspace of its own, so calls may overlap and
     be captured in CUDA graphs."""
     if not isinstance(x, torch.Tensor) or x.ndim != 2 or x.dtype not in (torch.bfloat16, torch.float16):
