@@ -404,3 +404,24 @@ def test_a_router_weight_that_is_not_bf16_is_refused(dtype):
     with pytest.raises(ValueError, match="bf16"):
         tb.moe_layer_tokens(x, wg.to(dtype), bg, lw, k)
     assert torch.isfinite(tb.moe_layer_tokens(x, tb.prepare_router_weight(wg.to(dtype)), bg, lw, k)).all()
+
+
+@gpu
+@pytest.mark.parametrize("T,E,k", [(16, 256, 16), (8, 128, 16), (16, 250, 15)])
+def test_every_pick_another_expert(T, E, k):
+    """as many active experts as there can be: the lists of experts are full"""
+    d, ff = 64, 32
+    lw, full1, full2 = make_layer(E, d, ff, 23)
+    g = torch.Generator(device="cuda").manual_seed(24)
+    x = torch.randn(T, d, device="cuda", generator=g) * 0.1
+    x[:, :T] = torch.eye(T, device="cuda") * 4
+    x = x.bfloat16()
+    wg = torch.randn(d, E, device="cuda", generator=g) * 0.01
+    experts = torch.randperm(E, device="cuda", generator=g)[:T * k].view(T, k)
+    for t in range(T):
+        wg[t, experts[t]] = 2.0 + torch.rand(k, device="cuda", generator=g)
+    wg = tb.prepare_router_weight(wg.bfloat16())
+    y = tb.moe_layer_tokens(x, wg, None, lw, k)
+    tb.matmul_check_status()
+    assert (x.double() @ wg.double()).topk(k, 1).indices.unique().numel() == T * k
+    check(y, *reference(x, wg, None, lw, full1, full2, k))
